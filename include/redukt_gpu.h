@@ -245,6 +245,103 @@ int32_t redukt_b200_forward_batch_cdf(uint32_t n_streams, const uint32_t* slots,
                                       const uint32_t* symbols, const uint32_t* cum_freqs, uint32_t* query_out,
                                       uint32_t* cdf_out);
 
+/* ---- Operators over a ragged batch of requests and a pool of state slots ----
+ *
+ * The calls below work on device memory only, need no model loaded, allocate nothing, keep nothing
+ * between calls and enqueue their work on cuda_stream (a cudaStream_t; NULL = the legacy default
+ * stream) without synchronising.  INVALID_ARGUMENT returns before any launch, with the reason in
+ * redukt_b200_last_error().  The first call on a device looks up that device's facts: make it
+ * before any stream capture.  What only the device can see (a slot out of range, a batch that does
+ * not fit) rejects its own request and sets bit 0 of the word read by redukt_b200_ops_error().
+ * Strides are in elements; a stride larger than its row is allowed.  Slots and requests: at most
+ * 4,096, as redukt_backend_batch_init. */
+#define REDUKT_DTYPE_F32 0
+#define REDUKT_DTYPE_BF16 1
+
+/* Waits for the current device, then reads and clears its operators' error word: bit 0 = a request
+ * was rejected, bit 1 = a bounded wait of a tensor-core kernel ran out (its outputs are invalid). */
+int32_t redukt_b200_ops_error(uint32_t* out_word);
+
+/* Plan of a ragged batch from the requests' lengths.  Request i has d_lengths[i] tokens and either
+ * continues the stream in slot d_want[i] or (UINT32_MAX) starts a new one; d_used[s] != 0 marks the
+ * slots in use.
+ *   d_cu[n + 1]           token offsets: prefix sums, none above max_tokens
+ *   d_slots[n]            the request's slot, UINT32_MAX = none.  A continuing request keeps the slot
+ *                         it names, the first of several that name it; the new requests that have
+ *                         tokens take the lowest slots that are neither in use nor named, in order.
+ *                         A request that ends above max_tokens gets none.
+ *   d_fresh[n]            1 = newly admitted: its slot's old contents are not its state
+ *   d_used_out[n_slots]   d_used with the named and the newly given slots marked (another buffer)
+ *   d_token_slot[max_tokens], d_token_pos[max_tokens]  each token's slot and position in its request
+ *   d_block_base[n + 1], d_blocks[max_blocks][2]  the requests cut into blocks of `block` tokens:
+ *                         first block of each request, and (request, index in it) of each block
+ * Entries past the last token or block are UINT32_MAX.  max_blocks must be at least
+ * max_tokens / block + n.  A request with tokens, or with a slot in d_want, that gets no slot is
+ * rejected (bit 0 of the error word); the others are planned as if it had a slot. */
+int32_t redukt_b200_plan_requests(const uint32_t* d_lengths, const uint32_t* d_want, uint32_t n, const uint8_t* d_used,
+                                  uint32_t n_slots, uint32_t block, uint32_t max_tokens, uint32_t max_blocks, uint32_t* d_cu,
+                                  uint32_t* d_slots, uint32_t* d_fresh, uint8_t* d_used_out, uint32_t* d_token_slot,
+                                  uint32_t* d_token_pos, uint32_t* d_block_base, uint32_t* d_blocks, void* cuda_stream);
+
+/* The gated delta rule for one token of each of n_streams streams.  Per value head h, with the
+ * query/key head h / (n_v_heads / n_qk_heads) and a = exp(log_decay):
+ *     S = a S + beta (v - a S k) k^T,   out = scale S q
+ * q, k: [n_streams][n_qk_heads][d_key]; v, out: [n_streams][n_v_heads][d_value], of type dtype;
+ * log_decay, beta: [n_streams][n_v_heads] f32 (row stride ld_gate).  With l2norm != 0, q and k are
+ * divided by sqrt(sum of squares + 1e-6) first.  The state is f32: d_state + slot * slot_stride
+ * holds [n_v_heads][d_value][d_key], updated in place; d_fresh[b] != 0 (d_fresh may be NULL) starts
+ * stream b from zero state.  A slot >= n_slots rejects its stream: its output row is zero and no
+ * state is touched.  Duplicate slots are the caller's responsibility.  d_key 64 or 128, d_value a
+ * multiple of 16 up to 256, the state on 16 bytes with slot_stride a multiple of 4. */
+int32_t redukt_b200_delta_step(const void* d_q, const void* d_k, const void* d_v, int32_t dtype, const float* d_log_decay,
+                               const float* d_beta, uint32_t n_streams, const uint32_t* d_slots, const uint32_t* d_fresh,
+                               uint32_t n_qk_heads, uint32_t n_v_heads, uint32_t d_key, uint32_t d_value, uint64_t ld_q,
+                               uint64_t ld_k, uint64_t ld_v, uint64_t ld_gate, uint64_t ld_out, float scale, int32_t l2norm,
+                               float* d_state, uint32_t n_slots, uint64_t slot_stride, void* d_out, void* cuda_stream);
+
+/* The gated delta rule over every token of each request: rows d_cu[i] .. d_cu[i + 1] of q, k, v,
+ * log_decay, beta and out belong to request i, whose state is in slot d_slots[i] (arguments
+ * otherwise as redukt_b200_delta_step).  n_tokens is the number of rows of the arrays; no row at or
+ * above it is touched.  A request without tokens keeps its state (fresh: zero state).  The same
+ * call gives the same bits every time; they are near, not equal to, n calls of delta_step.
+ * d_blocks (block, max_blocks) is the plan's block table, used to cut long requests where there are
+ * few of them; NULL = never cut.  d_work: redukt_b200_delta_work_bytes() bytes on 256; with less
+ * (NULL and 0 among it) requests are not cut. */
+int32_t redukt_b200_delta_chunk(const void* d_q, const void* d_k, const void* d_v, int32_t dtype, const float* d_log_decay,
+                                const float* d_beta, uint32_t n_tokens, uint32_t n_requests, const uint32_t* d_cu,
+                                const uint32_t* d_slots, const uint32_t* d_fresh, uint32_t n_qk_heads, uint32_t n_v_heads,
+                                uint32_t d_key, uint32_t d_value, uint64_t ld_q, uint64_t ld_k, uint64_t ld_v, uint64_t ld_gate,
+                                uint64_t ld_out, float scale, int32_t l2norm, float* d_state, uint32_t n_slots,
+                                uint64_t slot_stride, const uint32_t* d_blocks, uint32_t block, uint32_t max_blocks, void* d_out,
+                                void* d_work, uint64_t work_bytes, void* cuda_stream);
+
+/* Rows of k values of type dtype to int8 with one f32 scale per row: scale = max |x| * (1 / 127) (1 for
+ * a zero row), q = clamp(round half away from zero (x * (1 / scale)), -127, 127), NaN to 0; each step is
+ * one correctly rounded f32 operation, 1 / 127 a constant.  The RWKV-7 step's recipe
+ * (quantize_vec_i8_into, src/domain/tensor.rs:1791-1800) divides by 127 instead: its scale can differ
+ * in the last bit. */
+int32_t redukt_b200_quantize_tokens(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q,
+                                    uint64_t ld_q, float* d_scale, void* cuda_stream);
+
+/* out[t][c] = float(sum_k a[t][k] w[c][k]) * (w_scale[c] * a_scale[t]), the sum exact in int32
+ * (k < 131072), out of type out_dtype.  Rows of a and w start on 16 bytes (base and stride); what
+ * lies between k and the stride is not read as data.  Every size gives the same bits for a row. */
+int32_t redukt_b200_w8a8_matmul(const int8_t* d_a, uint64_t ld_a, const float* d_a_scale, uint32_t n_tokens, const int8_t* d_w,
+                                uint64_t ld_w, const float* d_w_scale, uint32_t n_out, uint32_t k, void* d_out, int32_t out_dtype,
+                                uint64_t ld_out, void* d_work, uint64_t work_bytes, void* cuda_stream);
+
+/* quantize_tokens then w8a8_matmul of its result: a linear layer on f32 or bf16 activations.
+ * d_work: redukt_b200_w8a8_work_bytes() bytes on 256. */
+int32_t redukt_b200_w8a8_linear(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, const int8_t* d_w,
+                                uint64_t ld_w, const float* d_w_scale, uint32_t n_out, void* d_out, int32_t out_dtype,
+                                uint64_t ld_out, void* d_work, uint64_t work_bytes, void* cuda_stream);
+
+/* Workspace of redukt_b200_w8a8_linear and redukt_b200_w8a8_matmul (matmul: may be NULL and 0). */
+uint64_t redukt_b200_w8a8_work_bytes(uint32_t n_tokens, uint32_t n_out, uint32_t k);
+
+/* Workspace with which redukt_b200_delta_chunk can cut requests (max_blocks of the block table). */
+uint64_t redukt_b200_delta_work_bytes(uint32_t max_blocks, uint32_t n_v_heads, uint32_t d_key, uint32_t d_value);
+
 /* Last error message of this library (empty string when none). */
 const char* redukt_b200_last_error(void);
 

@@ -8,24 +8,36 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libredukt_gpu.so")
-SOURCES = ["redukt_gpu.cu"]
-HEADERS = ["rk_math.cuh", "rk_kernels.cuh", "rk_fused.cuh", "rk_tc.cuh", "rk_rwkv7.cuh", "rwkv7_engine.cuh", "rk_cdf.cuh", "rk_exp_table.h"]
+# each source with the headers it is rebuilt for
+SOURCES = {
+    "redukt_gpu.cu": ["rk_math.cuh", "rk_kernels.cuh", "rk_fused.cuh", "rk_tc.cuh", "rk_rwkv7.cuh", "rwkv7_engine.cuh",
+                      "rk_cdf.cuh", "rk_exp_table.h", "rk_error.h"],
+    "rk_ops.cu": ["rk_error.h", "rk_plan.cuh", "rk_delta.cuh", "rk_w8a8.cuh"],
+}
+ABI = os.path.join(HERE, "..", "include", "redukt_gpu.h")
+OBJ = os.path.join(CSRC, "_build")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
-    "-lineinfo", "-O3", "-std=c++17", "--shared",
+    "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-Wall,-Wno-unused-function",
     "-Xptxas", "-warn-spills",
 ]
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB):
+def _newer(paths, than: str) -> bool:
+    if not os.path.exists(than):
         return True
-    t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    deps.append(os.path.join(HERE, "..", "include", "redukt_gpu.h"))
-    return any(os.path.exists(p) and os.path.getmtime(p) > t for p in deps)
+    t = os.path.getmtime(than)
+    return any(os.path.exists(p) and os.path.getmtime(p) > t for p in paths)
+
+
+def _deps(src: str) -> list:
+    return [os.path.join(CSRC, f) for f in [src, *SOURCES[src]]] + [ABI]
+
+
+def _stale() -> bool:
+    return any(_newer(_deps(s), LIB) for s in SOURCES)
 
 
 ARC_LIB = os.path.join(HERE, "libredukt_archive.so")
@@ -52,15 +64,30 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
         return LIB
     nvcc = os.environ.get("NVCC", "nvcc")
-    cmd = [nvcc, *NVCC_FLAGS, "-o", LIB + ".tmp", *[os.path.join(CSRC, s) for s in SOURCES]]
-    if verbose:
-        cmd.insert(-len(SOURCES) - 2, "-Xptxas=-v")
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    os.makedirs(OBJ, exist_ok=True)
+    objs, running = [], []
+    for src in SOURCES:   # the sources compile side by side; an object is kept until one of its files changes
+        obj = os.path.join(OBJ, os.path.splitext(src)[0] + ".o")
+        objs.append(obj)
+        if not force and not _newer(_deps(src), obj):
+            continue
+        cmd = [nvcc, *NVCC_FLAGS, *(["-Xptxas=-v"] if verbose else []), "-c", "-o", obj + ".tmp", os.path.join(CSRC, src)]
+        running.append((src, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    failed = []
+    for src, obj, proc in running:
+        said = proc.communicate()[0]
+        if proc.returncode != 0 or verbose:
+            sys.stderr.write(said)
+        if proc.returncode != 0:
+            failed.append(src)
+        else:
+            os.replace(obj + ".tmp", obj)
+    if failed:
+        raise RuntimeError("nvcc failed building " + ", ".join(failed))
+    r = subprocess.run([nvcc, *NVCC_FLAGS, "--shared", "-o", LIB + ".tmp", *objs], capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError("nvcc failed building libredukt_gpu.so")
-    if verbose:
-        sys.stderr.write(r.stderr)
+        raise RuntimeError("nvcc failed linking libredukt_gpu.so")
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

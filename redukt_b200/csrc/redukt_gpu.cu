@@ -24,6 +24,20 @@
 #include "rk_rwkv7.cuh"
 #include "rk_tc.cuh"
 #include "rk_cdf.cuh"
+#include "rk_error.h"
+
+namespace {
+char g_err[1024] = "";
+}
+
+// The message of redukt_b200_last_error(), for every translation unit of the library.
+void rk::set_err(const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    fprintf(stderr, "[redukt-b200] %s\n", g_err);
+}
 
 namespace {
 
@@ -38,16 +52,6 @@ constexpr uint32_t kFlagQ8Payload = 1u << 6;  // Q8 matrices stored as int8 + gr
 constexpr uint32_t kMaxStreams = 4096u;  // batch_init cap (mamba_cuda.cu:55)
 
 enum Profile { kF32 = 0, kQ8 = 1, kQ8Row = 2 };
-
-char g_err[1024] = "";
-
-void set_err(const char* fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof(g_err), fmt, ap);
-    va_end(ap);
-    fprintf(stderr, "[redukt-b200] %s\n", g_err);
-}
 
 #define CK(call, code)                                                                        \
     do {                                                                                      \

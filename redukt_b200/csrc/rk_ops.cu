@@ -1,0 +1,289 @@
+// The ragged-batch operators' entry points (include/redukt_gpu.h): argument checks and launches.
+// They need no model loaded, allocate nothing and keep nothing between calls; every launch goes
+// to the caller's stream.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+
+#include "../../include/redukt_gpu.h"
+#include "rk_delta.cuh"
+#include "rk_error.h"
+#include "rk_plan.cuh"
+#include "rk_w8a8.cuh"
+
+namespace {
+
+using rk::set_err;
+
+#define OP_CK(call)                                                                                     \
+    do {                                                                                                \
+        cudaError_t e_ = (call);                                                                        \
+        if (e_ != cudaSuccess) {                                                                        \
+            set_err("CUDA error %s at %s:%d (%s)", cudaGetErrorString(e_), __FILE__, __LINE__, #call);  \
+            return BACKEND_FORWARD_FAILED;                                                              \
+        }                                                                                               \
+    } while (0)
+
+#define OP_REQUIRE(cond, ...)                       \
+    do {                                            \
+        if (!(cond)) {                              \
+            set_err(__VA_ARGS__);                   \
+            return BACKEND_INVALID_ARGUMENT;        \
+        }                                           \
+    } while (0)
+
+// The operators' error word: a fixed word in the library's own device memory, one per device.
+__device__ uint32_t g_ops_err = 0;
+
+constexpr int kMaxDevices = 64;
+struct Device {
+    std::mutex mu;
+    bool ready = false;
+    uint32_t* err = nullptr;
+    int sms = 0;
+};
+Device g_device[kMaxDevices];
+
+// The current device's facts; the first call on a device looks them up and sets the kernels'
+// shared-memory limits.
+int32_t device(Device** out) {
+    int dev = -1;
+    OP_CK(cudaGetDevice(&dev));
+    OP_REQUIRE(dev >= 0 && dev < kMaxDevices, "device ordinal %d is out of range", dev);
+    Device& d = g_device[dev];
+    std::lock_guard<std::mutex> lock(d.mu);
+    if (!d.ready) {
+        void* p = nullptr;
+        OP_CK(cudaGetSymbolAddress(&p, g_ops_err));
+        d.err = static_cast<uint32_t*>(p);
+        OP_CK(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
+        OP_CK(cudaFuncSetAttribute(rk::plan::k_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::plan::Smem)));
+        d.ready = true;
+    }
+    *out = &d;
+    return BACKEND_OK;
+}
+
+cudaStream_t stream_of(void* s) { return reinterpret_cast<cudaStream_t>(s); }
+uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+size_t dtype_size(int32_t t) { return t == REDUKT_DTYPE_F32 ? 4 : t == REDUKT_DTYPE_BF16 ? 2 : 0; }
+
+// ---- gated delta rule ----
+
+int32_t delta_args(const char* what, rk::delta::Args& a, const void* d_q, const void* d_k, const void* d_v, int32_t dtype,
+                   const float* d_log_decay, const float* d_beta, const uint32_t* d_slots, const uint32_t* d_fresh, uint32_t n,
+                   uint32_t n_rows, uint32_t n_qk_heads, uint32_t n_v_heads, uint32_t d_key, uint32_t d_value, uint64_t ld_q,
+                   uint64_t ld_k, uint64_t ld_v, uint64_t ld_gate, uint64_t ld_out, float scale, int32_t l2norm, float* d_state,
+                   uint32_t n_slots, uint64_t slot_stride, void* d_out) {
+    const size_t es = dtype_size(dtype);
+    OP_REQUIRE(es != 0, "%s: dtype %d is neither f32 (0) nor bf16 (1)", what, dtype);
+    OP_REQUIRE(n <= 4096, "%s: %u requests (at most 4096)", what, n);
+    OP_REQUIRE(n_qk_heads > 0 && n_v_heads > 0 && n_v_heads % n_qk_heads == 0 && n_v_heads <= 4096,
+               "%s: %u value heads are not a multiple of %u query/key heads (at most 4096)", what, n_v_heads, n_qk_heads);
+    OP_REQUIRE(d_key == 64 || d_key == 128, "%s: key size %u (64 or 128)", what, d_key);
+    OP_REQUIRE(d_value >= 16 && d_value <= 256 && d_value % 16 == 0, "%s: value size %u (a multiple of 16 up to 256)", what, d_value);
+    OP_REQUIRE(ld_q >= (uint64_t)n_qk_heads * d_key && ld_k >= (uint64_t)n_qk_heads * d_key &&
+                   ld_v >= (uint64_t)n_v_heads * d_value && ld_out >= (uint64_t)n_v_heads * d_value && ld_gate >= n_v_heads,
+               "%s: a row stride is smaller than its row", what);
+    OP_REQUIRE(slot_stride >= (uint64_t)n_v_heads * d_value * d_key && slot_stride % 4 == 0,
+               "%s: slot stride %llu (at least the slot's floats, a multiple of 4)", what, (unsigned long long)slot_stride);
+    if (n == 0) return BACKEND_OK;
+    OP_REQUIRE(d_slots && d_state && (n_rows == 0 || (d_q && d_k && d_v && d_log_decay && d_beta && d_out)), "%s: NULL argument", what);
+    OP_REQUIRE(aligned(d_state, 16), "%s: the state is not 16-byte aligned", what);
+    OP_REQUIRE(aligned(d_q, es) && aligned(d_k, es) && aligned(d_v, es) && aligned(d_out, es) && aligned(d_log_decay, 4) &&
+                   aligned(d_beta, 4), "%s: misaligned pointer", what);
+    OP_REQUIRE(std::isfinite(scale), "%s: the scale is not finite", what);
+    a = {d_q, d_k, d_v, d_log_decay, d_beta, nullptr, d_slots, d_fresh, n, n_rows, n_qk_heads, n_v_heads, d_value,
+         ld_q, ld_k, ld_v, ld_gate, ld_out, scale, l2norm, d_state, n_slots, slot_stride, d_out, nullptr};
+    return BACKEND_OK;
+}
+
+// ---- 8-bit product ----
+
+int32_t w8_check(const char* what, uint32_t n_tokens, uint32_t n_out, uint32_t k, uint64_t ld_w, const void* d_w,
+                 const void* d_w_scale, const void* d_out, int32_t out_dtype, uint64_t ld_out) {
+    OP_REQUIRE(dtype_size(out_dtype) != 0, "%s: dtype %d is neither f32 (0) nor bf16 (1)", what, out_dtype);
+    OP_REQUIRE(k > 0 && k < 131072, "%s: k %u (1 to 131071: the sum is exact in 32 bits)", what, k);
+    OP_REQUIRE(n_tokens <= 0x7FFFFFFFu && n_out <= 0x7FFFFFFFu, "%s: too many rows", what);
+    OP_REQUIRE(ld_w >= k && ld_w % 16 == 0 && aligned(d_w, 16), "%s: int8 rows must start on 16 bytes and hold k values", what);
+    OP_REQUIRE(ld_out >= n_out, "%s: a row stride is smaller than its row", what);
+    OP_REQUIRE(n_tokens == 0 || n_out == 0 || (d_w && d_w_scale && d_out), "%s: NULL argument", what);
+    OP_REQUIRE(aligned(d_out, dtype_size(out_dtype)) && aligned(d_w_scale, 4), "%s: misaligned pointer", what);
+    return BACKEND_OK;
+}
+
+int32_t quantize(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q, uint64_t ld_q,
+                 float* d_scale, cudaStream_t st) {
+    if (dtype == REDUKT_DTYPE_F32)
+        rk::w8::k_quant_tokens<float><<<n_tokens, 256, 0, st>>>((const float*)d_x, k, ld_x, d_q, ld_q, d_scale);
+    else
+        rk::w8::k_quant_tokens<__nv_bfloat16><<<n_tokens, 256, 0, st>>>((const __nv_bfloat16*)d_x, k, ld_x, d_q, ld_q, d_scale);
+    OP_CK(cudaGetLastError());
+    return BACKEND_OK;
+}
+
+int32_t matmul(const rk::w8::Args& a, int32_t out_dtype, cudaStream_t st) {
+    const dim3 grid((unsigned)ceil_div(a.n, 64), (unsigned)ceil_div(a.m, 64));
+    if (out_dtype == REDUKT_DTYPE_F32) rk::w8::k_w8a8_dp4a<float><<<grid, 256, 0, st>>>(a);
+    else rk::w8::k_w8a8_dp4a<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
+    OP_CK(cudaGetLastError());
+    return BACKEND_OK;
+}
+
+uint64_t quant_ld(uint32_t k) { return ceil_div(k, 16) * 16; }
+uint64_t quant_bytes(uint32_t n_tokens, uint32_t k) { return ceil_div((uint64_t)n_tokens * quant_ld(k), 256) * 256 + ceil_div(4ull * n_tokens, 256) * 256; }
+
+}  // namespace
+
+extern "C" {
+
+int32_t redukt_b200_ops_error(uint32_t* out_word) {
+    if (!out_word) return BACKEND_INVALID_ARGUMENT;
+    Device* d = nullptr;
+    if (int32_t rc = device(&d)) return rc;
+    OP_CK(cudaDeviceSynchronize());
+    OP_CK(cudaMemcpy(out_word, d->err, 4, cudaMemcpyDeviceToHost));
+    OP_CK(cudaMemset(d->err, 0, 4));
+    return BACKEND_OK;
+}
+
+int32_t redukt_b200_plan_requests(const uint32_t* d_lengths, const uint32_t* d_want, uint32_t n, const uint8_t* d_used,
+                                  uint32_t n_slots, uint32_t block, uint32_t max_tokens, uint32_t max_blocks, uint32_t* d_cu,
+                                  uint32_t* d_slots, uint32_t* d_fresh, uint8_t* d_used_out, uint32_t* d_token_slot,
+                                  uint32_t* d_token_pos, uint32_t* d_block_base, uint32_t* d_blocks, void* cuda_stream) {
+    OP_REQUIRE(n <= rk::plan::kMax && n_slots <= rk::plan::kMax, "plan_requests: %u requests over %u slots (at most 4096 each)", n, n_slots);
+    OP_REQUIRE(block > 0, "plan_requests: block size 0");
+    OP_REQUIRE((uint64_t)max_tokens / block + n <= max_blocks, "plan_requests: max_blocks %u is below max_tokens / block + n", max_blocks);
+    OP_REQUIRE(d_cu && d_block_base && (n == 0 || (d_lengths && d_want && d_slots && d_fresh)) && (n_slots == 0 || (d_used && d_used_out)) &&
+                   (max_tokens == 0 || (d_token_slot && d_token_pos)) && (max_blocks == 0 || d_blocks),
+               "plan_requests: NULL argument");
+    OP_REQUIRE(d_used != d_used_out || n_slots == 0, "plan_requests: used and used_out are the same buffer");
+    Device* d = nullptr;
+    if (int32_t rc = device(&d)) return rc;
+    rk::plan::Args a = {d_lengths, d_want, d_used, n, n_slots, block, max_tokens, max_blocks, d_cu, d_slots, d_fresh, d_used_out,
+                        d_token_slot, d_token_pos, d_block_base, d_blocks, d->err};
+    // every block repeats the scans, so a block is worth adding only with a few thousand tokens to fill
+    const uint64_t fill = std::max<uint64_t>(ceil_div(max_tokens, 8192), ceil_div(max_blocks, 4096));
+    const unsigned grid = (unsigned)std::min<uint64_t>(std::max<uint64_t>(fill, 1), (uint64_t)d->sms);
+    rk::plan::k_plan<<<grid, rk::plan::kThreads, sizeof(rk::plan::Smem), stream_of(cuda_stream)>>>(a);
+    OP_CK(cudaGetLastError());
+    return BACKEND_OK;
+}
+
+int32_t redukt_b200_delta_step(const void* d_q, const void* d_k, const void* d_v, int32_t dtype, const float* d_log_decay,
+                               const float* d_beta, uint32_t n_streams, const uint32_t* d_slots, const uint32_t* d_fresh,
+                               uint32_t n_qk_heads, uint32_t n_v_heads, uint32_t d_key, uint32_t d_value, uint64_t ld_q,
+                               uint64_t ld_k, uint64_t ld_v, uint64_t ld_gate, uint64_t ld_out, float scale, int32_t l2norm,
+                               float* d_state, uint32_t n_slots, uint64_t slot_stride, void* d_out, void* cuda_stream) {
+    rk::delta::Args a{};
+    if (int32_t rc = delta_args("delta_step", a, d_q, d_k, d_v, dtype, d_log_decay, d_beta, d_slots, d_fresh, n_streams, n_streams,
+                                n_qk_heads, n_v_heads, d_key, d_value, ld_q, ld_k, ld_v, ld_gate, ld_out, scale, l2norm, d_state,
+                                n_slots, slot_stride, d_out))
+        return rc;
+    if (n_streams == 0) return BACKEND_OK;
+    Device* d = nullptr;
+    if (int32_t rc = device(&d)) return rc;
+    a.err = d->err;
+    const dim3 grid((d_value + rk::delta::kRows - 1) / rk::delta::kRows, n_v_heads, n_streams);
+    const cudaStream_t st = stream_of(cuda_stream);
+    const int threads = rk::delta::kWarps * 32;
+    if (dtype == REDUKT_DTYPE_F32) {
+        if (d_key == 64) rk::delta::k_delta_step<64, float><<<grid, threads, 0, st>>>(a);
+        else rk::delta::k_delta_step<128, float><<<grid, threads, 0, st>>>(a);
+    } else {
+        if (d_key == 64) rk::delta::k_delta_step<64, __nv_bfloat16><<<grid, threads, 0, st>>>(a);
+        else rk::delta::k_delta_step<128, __nv_bfloat16><<<grid, threads, 0, st>>>(a);
+    }
+    OP_CK(cudaGetLastError());
+    return BACKEND_OK;
+}
+
+int32_t redukt_b200_delta_chunk(const void* d_q, const void* d_k, const void* d_v, int32_t dtype, const float* d_log_decay,
+                                const float* d_beta, uint32_t n_tokens, uint32_t n_requests, const uint32_t* d_cu,
+                                const uint32_t* d_slots, const uint32_t* d_fresh, uint32_t n_qk_heads, uint32_t n_v_heads,
+                                uint32_t d_key, uint32_t d_value, uint64_t ld_q, uint64_t ld_k, uint64_t ld_v, uint64_t ld_gate,
+                                uint64_t ld_out, float scale, int32_t l2norm, float* d_state, uint32_t n_slots,
+                                uint64_t slot_stride, const uint32_t* d_blocks, uint32_t block, uint32_t max_blocks, void* d_out,
+                                void* d_work, uint64_t work_bytes, void* cuda_stream) {
+    rk::delta::Args a{};
+    if (int32_t rc = delta_args("delta_chunk", a, d_q, d_k, d_v, dtype, d_log_decay, d_beta, d_slots, d_fresh, n_requests, n_tokens,
+                                n_qk_heads, n_v_heads, d_key, d_value, ld_q, ld_k, ld_v, ld_gate, ld_out, scale, l2norm, d_state,
+                                n_slots, slot_stride, d_out))
+        return rc;
+    if (n_requests == 0) return BACKEND_OK;
+    OP_REQUIRE(d_cu, "delta_chunk: NULL argument");
+    OP_REQUIRE(!d_blocks || (block > 0 && block % 64 == 0 && (uint64_t)n_tokens / block + n_requests <= max_blocks),
+               "delta_chunk: a block table needs a block of a multiple of 64 tokens and max_blocks of n_tokens / block + n_requests");
+    OP_REQUIRE(!d_work || aligned(d_work, 256), "delta_chunk: the workspace is not 256-byte aligned");
+    Device* d = nullptr;
+    if (int32_t rc = device(&d)) return rc;
+    a.err = d->err;
+    a.cu = d_cu;
+    const dim3 grid((d_value + rk::delta::kRows - 1) / rk::delta::kRows, n_v_heads, n_requests);
+    const cudaStream_t st = stream_of(cuda_stream);
+    const int threads = rk::delta::kWarps * 32;
+    if (dtype == REDUKT_DTYPE_F32) {
+        if (d_key == 64) rk::delta::k_delta_serial<64, float><<<grid, threads, 0, st>>>(a);
+        else rk::delta::k_delta_serial<128, float><<<grid, threads, 0, st>>>(a);
+    } else {
+        if (d_key == 64) rk::delta::k_delta_serial<64, __nv_bfloat16><<<grid, threads, 0, st>>>(a);
+        else rk::delta::k_delta_serial<128, __nv_bfloat16><<<grid, threads, 0, st>>>(a);
+    }
+    OP_CK(cudaGetLastError());
+    return BACKEND_OK;
+}
+
+int32_t redukt_b200_quantize_tokens(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q,
+                                    uint64_t ld_q, float* d_scale, void* cuda_stream) {
+    OP_REQUIRE(dtype_size(dtype) != 0, "quantize_tokens: dtype %d is neither f32 (0) nor bf16 (1)", dtype);
+    OP_REQUIRE(k > 0 && k < 131072 && n_tokens <= 0x7FFFFFFFu, "quantize_tokens: %u tokens of %u values (1 to 131071)", n_tokens, k);
+    OP_REQUIRE(ld_x >= k && ld_q >= k, "quantize_tokens: a row stride is smaller than its row");
+    if (n_tokens == 0) return BACKEND_OK;
+    OP_REQUIRE(d_x && d_q && d_scale, "quantize_tokens: NULL argument");
+    OP_REQUIRE(aligned(d_x, dtype_size(dtype)) && aligned(d_scale, 4), "quantize_tokens: misaligned pointer");
+    return quantize(d_x, dtype, n_tokens, k, ld_x, d_q, ld_q, d_scale, stream_of(cuda_stream));
+}
+
+uint64_t redukt_b200_delta_work_bytes(uint32_t max_blocks, uint32_t n_v_heads, uint32_t d_key, uint32_t d_value) {
+    (void)max_blocks, (void)n_v_heads, (void)d_key, (void)d_value;
+    return 0;
+}
+
+uint64_t redukt_b200_w8a8_work_bytes(uint32_t n_tokens, uint32_t n_out, uint32_t k) {
+    (void)n_out;
+    return quant_bytes(n_tokens, k);
+}
+
+int32_t redukt_b200_w8a8_matmul(const int8_t* d_a, uint64_t ld_a, const float* d_a_scale, uint32_t n_tokens, const int8_t* d_w,
+                                uint64_t ld_w, const float* d_w_scale, uint32_t n_out, uint32_t k, void* d_out, int32_t out_dtype,
+                                uint64_t ld_out, void* d_work, uint64_t work_bytes, void* cuda_stream) {
+    if (int32_t rc = w8_check("w8a8_matmul", n_tokens, n_out, k, ld_w, d_w, d_w_scale, d_out, out_dtype, ld_out)) return rc;
+    if (n_tokens == 0 || n_out == 0) return BACKEND_OK;
+    OP_REQUIRE(d_a && d_a_scale, "w8a8_matmul: NULL argument");
+    OP_REQUIRE(ld_a >= k && ld_a % 16 == 0 && aligned(d_a, 16) && aligned(d_a_scale, 4), "w8a8_matmul: int8 rows must start on 16 bytes and hold k values");
+    rk::w8::Args a = {d_a, d_a_scale, d_w, d_w_scale, ld_a, ld_w, ld_out, n_tokens, n_out, k, d_out};
+    return matmul(a, out_dtype, stream_of(cuda_stream));
+}
+
+int32_t redukt_b200_w8a8_linear(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, const int8_t* d_w,
+                                uint64_t ld_w, const float* d_w_scale, uint32_t n_out, void* d_out, int32_t out_dtype,
+                                uint64_t ld_out, void* d_work, uint64_t work_bytes, void* cuda_stream) {
+    OP_REQUIRE(dtype_size(dtype) != 0, "w8a8_linear: dtype %d is neither f32 (0) nor bf16 (1)", dtype);
+    if (int32_t rc = w8_check("w8a8_linear", n_tokens, n_out, k, ld_w, d_w, d_w_scale, d_out, out_dtype, ld_out)) return rc;
+    if (n_tokens == 0 || n_out == 0) return BACKEND_OK;
+    OP_REQUIRE(d_x && ld_x >= k && aligned(d_x, dtype_size(dtype)), "w8a8_linear: the activations are NULL, misaligned or narrower than k");
+    OP_REQUIRE(d_work && aligned(d_work, 256) && work_bytes >= redukt_b200_w8a8_work_bytes(n_tokens, n_out, k),
+               "w8a8_linear: the workspace needs %llu bytes on 256", (unsigned long long)redukt_b200_w8a8_work_bytes(n_tokens, n_out, k));
+    int8_t* q = static_cast<int8_t*>(d_work);
+    float* s = reinterpret_cast<float*>(q + ceil_div((uint64_t)n_tokens * quant_ld(k), 256) * 256);
+    const cudaStream_t st = stream_of(cuda_stream);
+    if (int32_t rc = quantize(d_x, dtype, n_tokens, k, ld_x, q, quant_ld(k), s, st)) return rc;
+    rk::w8::Args a = {q, s, d_w, d_w_scale, quant_ld(k), ld_w, ld_out, n_tokens, n_out, k, d_out};
+    return matmul(a, out_dtype, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,402 @@
+"""delta_chunk and delta_step against the recurrence in 64 bits.
+
+Tolerances (relative 2-norm over one request's outputs or state, u = 2^-24): a product of length d
+in f32 is off by at most d u times the norms of its factors and by about sqrt(d) u in practice, and
+the rule's transition a (I - b k k^T) does not expand for |k| <= 1, 0 <= b <= 1, a <= 1, so errors of
+different tokens add like independent ones: sqrt(1000 tokens * 128) u = 2.1e-5.  F32 = 2e-5.  A bf16
+output rounds that once more, by at most 2^-8 of each element (8 significant bits, to nearest)."""
+import numpy as np
+import pytest
+
+from redukt_b200 import build as B
+from redukt_b200.plugin import DTYPE_BF16, DTYPE_F32, BackendResult, PluginLibrary
+
+NONE = 0xFFFFFFFF
+F32, BF16 = 2e-5, 2.0 ** -8
+
+
+@pytest.fixture(scope="module")
+def lib():
+    B.build()
+    return PluginLibrary()
+
+
+def rule(q, k, v, g, beta, S, scale, l2norm):
+    """One request: q, k [T, hk, dk], v [T, hv, dv], g, beta [T, hv], S [hv, dv, dk], all float64."""
+    group = v.shape[1] // q.shape[1]
+    q, k = np.repeat(q, group, 1), np.repeat(k, group, 1)
+    if l2norm:
+        q, k = (x / np.sqrt((x * x).sum(-1, keepdims=True) + 1e-6) for x in (q, k))
+    S, out = S.copy(), np.zeros(v.shape)
+    for t in range(len(v)):
+        S *= np.exp(g[t])[:, None, None]
+        u = beta[t][:, None] * (v[t] - np.einsum("hvk,hk->hv", S, k[t]))
+        S += u[:, :, None] * k[t][:, None, :]
+        out[t] = scale * np.einsum("hvk,hk->hv", S, q[t])
+    return out, S
+
+
+def off_by(got, want):
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    n = np.linalg.norm(want)
+    return 0.0 if not got.size else float(np.linalg.norm(got - want) / n) if n else float(np.linalg.norm(got))
+
+
+def fits(got, want, dtype):
+    """Outputs of one request and head: within F32 in 2-norm, for bf16 each element within its own
+    rounding of a value that may be off by F32 of the whole."""
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    if dtype == DTYPE_F32:
+        return off_by(got, want) <= F32
+    return bool((np.abs(got - want) <= BF16 * np.abs(want) + (1 + BF16) * F32 * np.linalg.norm(want)).all())
+
+
+class Batch:
+    """Inputs on the GPU in one layout, and the reference's answer for them."""
+
+    def __init__(self, lens, hk=2, hv=2, dk=64, dv=64, dtype=DTYPE_F32, l2norm=True, seed=0, pad=0, off=0, slots=None, fresh=None,
+                 n_slots=None, gate=None, beta=None, key_scale=1.0, extra_rows=0, scale=0.25):
+        import torch
+        r = np.random.default_rng(seed)
+        n, T = len(lens), int(sum(lens))
+        self.lens, self.hk, self.hv, self.dk, self.dv, self.dtype, self.l2norm, self.scale = lens, hk, hv, dk, dv, dtype, l2norm, scale
+        self.n, self.T, self.rows = n, T, T + extra_rows
+        self.n_slots = n_slots or n + 2
+        self.slots = np.asarray(r.permutation(self.n_slots)[:n] if slots is None else slots, np.uint32)
+        self.fresh = np.asarray(r.integers(0, 2, n) if fresh is None else fresh, np.uint32)
+        self.tdt = torch.bfloat16 if dtype == DTYPE_BF16 else torch.float32
+        q, k, v = (r.standard_normal((T, h, d)) for h, d in ((hk, dk), (hk, dk), (hv, dv)))
+        if not l2norm:
+            k /= np.sqrt((k * k).sum(-1, keepdims=True))
+            q /= np.sqrt((q * q).sum(-1, keepdims=True))
+        k = k * key_scale
+        g = -np.exp(r.uniform(-6, 0.5, (T, hv))) if gate is None else gate(r, T, hv)
+        b = 1 / (1 + np.exp(-r.standard_normal((T, hv)))) if beta is None else beta(r, T, hv)
+        self.cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.uint32)
+
+        def lay(x, gate_like=False):
+            """[rows, w] at stride w + pad, `off` elements into a buffer of NaN."""
+            x = x.reshape(T, -1)
+            t = torch.float32 if gate_like else self.tdt
+            ld = x.shape[1] + pad
+            flat = torch.full((self.rows * ld + off + 64,), float("nan"), dtype=t, device="cuda")
+            view = flat[off:off + self.rows * ld].view(self.rows, ld)
+            view[:T, :x.shape[1]] = torch.from_numpy(np.ascontiguousarray(x, np.float32)).cuda().to(t)
+            return flat, view, ld
+
+        self.q, self.k, self.v = lay(q), lay(k), lay(v)
+        self.g, self.b = lay(g, True), lay(b, True)
+        self.state = (torch.randn(self.n_slots, hv, dv, dk, generator=torch.Generator().manual_seed(seed)) * 0.3).cuda()
+        self.host = [x[1][:T, :w].double().cpu().numpy().reshape(T, h, -1) for x, w, h in
+                     ((self.q, hk * dk, hk), (self.k, hk * dk, hk), (self.v, hv * dv, hv), (self.g, hv, hv), (self.b, hv, hv))]
+        self.host[3], self.host[4] = self.host[3].reshape(T, hv), self.host[4].reshape(T, hv)
+
+    def u32(self, x):
+        import torch
+        return torch.from_numpy(np.asarray(x, np.uint32).view(np.int32).copy()).cuda()
+
+    def reference(self):
+        """(outputs [T, hv, dv], states [n_slots, hv, dv, dk]) in float64."""
+        st = self.state.double().cpu().numpy()
+        out = np.zeros((self.T, self.hv, self.dv))
+        for i in range(self.n):
+            if self.slots[i] >= self.n_slots:
+                continue
+            a, b = self.cu[i], self.cu[i + 1]
+            S = np.zeros_like(st[0]) if self.fresh[i] else st[self.slots[i]]
+            out[a:b], st[self.slots[i]] = rule(*(x[a:b] for x in self.host), S, self.scale, self.l2norm)
+        return out, st
+
+    def out_buffer(self):
+        import torch
+        ld = self.hv * self.dv + 5
+        return torch.full((self.rows, ld), -7.0, dtype=self.tdt, device="cuda"), ld
+
+    def run(self, lib, step=False, cut=0, stream=0, state=None, use_fresh=True):
+        """-> (outputs as f32 numpy [T, hv, dv], states numpy); checks that nothing else was written."""
+        import torch
+        state = self.state.clone() if state is None else state
+        out, ldo = self.out_buffer()
+        slots, fresh = self.u32(self.slots), self.u32(self.fresh)
+        common = [self.q[1].data_ptr(), self.k[1].data_ptr(), self.v[1].data_ptr(), self.dtype, self.g[1].data_ptr(), self.b[1].data_ptr()]
+        tail = [self.hk, self.hv, self.dk, self.dv, self.q[2], self.k[2], self.v[2], self.g[2], ldo, self.scale, int(self.l2norm),
+                state.data_ptr(), self.n_slots, state.stride(0)]
+        f = fresh.data_ptr() if use_fresh else 0
+        if step:
+            torch.cuda.synchronize()
+            rc = lib.delta_step(*common, self.n, slots.data_ptr(), f, *tail, out.data_ptr(), stream)
+        else:
+            cu = self.u32(self.cu)
+            table, most, work = None, 0, None
+            if cut:
+                most = self.T // cut + self.n
+                rows = [(i, j) for i in range(self.n) for j in range(-(-int(self.lens[i]) // cut))]
+                table = self.u32(rows + [(NONE, NONE)] * (most - len(rows)))
+                work = torch.full((lib.delta_work_bytes(most, self.hv, self.dk, self.dv) + 256,), 0xFF, dtype=torch.uint8, device="cuda")
+            torch.cuda.synchronize()
+            rc = lib.delta_chunk(*common, self.rows, self.n, cu.data_ptr(), slots.data_ptr(), f, *tail,
+                                 table.data_ptr() if cut else 0, cut, most, out.data_ptr(), work.data_ptr() if cut else 0,
+                                 work.numel() if cut else 0, stream)
+        assert rc == BackendResult.OK, lib.last_error()
+        self.word = lib.ops_error()
+        h = out.float().cpu().numpy()
+        w = self.hv * self.dv
+        assert (h[:, w:] == -7.0).all() and (h[self.T:] == -7.0).all()
+        return h[:self.T, :w].reshape(self.T, self.hv, self.dv), state.cpu().numpy()
+
+    def check(self, lib, **kw):
+        want, wst = self.reference()
+        out, st = self.run(lib, **kw)
+        for i in range(self.n):
+            a, b = self.cu[i], self.cu[i + 1]
+            for h in range(self.hv):
+                assert fits(out[a:b, h], want[a:b, h], self.dtype), (i, h, self.lens[i], off_by(out[a:b, h], want[a:b, h]))
+                if self.slots[i] < self.n_slots:
+                    s = self.slots[i]
+                    assert off_by(st[s, h], wst[s, h]) <= F32, (i, h, self.lens[i], off_by(st[s, h], wst[s, h]))
+        idle = [s for s in range(self.n_slots) if s not in set(self.slots.tolist())]
+        before = self.state.cpu().numpy()
+        assert np.array_equal(st[idle].view(np.uint32), before[idle].view(np.uint32))
+        return out, st
+
+
+LENS = [[1], [2, 0, 3], [63, 64, 65], [15, 16, 17, 31, 33], [128, 1, 0, 200], [257]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", LENS, ids=str)
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_chunk_lengths(lib, lens, dtype, dk):
+    Batch(lens, dk=dk, dtype=dtype, seed=len(lens) + dk).check(lib)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hk,hv", [(1, 1), (1, 3), (2, 8), (5, 5)])
+@pytest.mark.parametrize("dv", [16, 48, 64, 128, 144, 256])
+def test_chunk_heads(lib, hk, hv, dv):
+    for dk, dtype in ((64, DTYPE_F32), (128, DTYPE_BF16), (128, DTYPE_F32)):
+        Batch([70, 9], hk=hk, hv=hv, dk=dk, dv=dv, dtype=dtype, l2norm=bool(hv % 2), seed=dv).check(lib)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128)])
+def test_chunk_long(lib, dtype, dk, dv):
+    Batch([1000, 130], hk=1, hv=2, dk=dk, dv=dv, dtype=dtype, seed=9).check(lib)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cut", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (64, 144)])
+def test_chunk_cut_requests(lib, cut, dtype, dk, dv):
+    """Few requests, long ones, with the block table that lets them be cut."""
+    Batch([900], hk=1, hv=2, dk=dk, dv=dv, dtype=dtype, seed=cut).check(lib, cut=cut)
+    Batch([513, 0, 1, 300], hk=1, hv=1, dk=dk, dv=dv, dtype=dtype, seed=cut + 1).check(lib, cut=cut)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("pad,off", [(0, 1), (8, 0), (3, 0), (3, 5)])
+def test_chunk_strides_and_alignment(lib, dtype, dk, pad, off):
+    Batch([66, 30], dk=dk, dv=64, dtype=dtype, pad=pad, off=off, extra_rows=3, seed=pad + off).check(lib)
+    Batch([1] * 5, dk=dk, dv=80, dtype=dtype, pad=pad, off=off, seed=pad + off).check(lib, step=True)
+
+
+def resets(r, T, h):
+    g = -np.exp(r.uniform(-6, 0.5, (T, h)))
+    g[r.random((T, h)) < 0.1] = -np.inf      # forget everything
+    g[r.random((T, h)) < 0.1] = 0.0
+    return g
+
+
+GATES = {"resets": resets, "none": lambda r, T, h: np.zeros((T, h)), "all": lambda r, T, h: np.full((T, h), -np.inf),
+         "strong": lambda r, T, h: -r.uniform(20, 90, (T, h)), "lowest": lambda r, T, h: np.full((T, h), -3.4e38),
+         "growing": lambda r, T, h: np.full((T, h), 0.01)}
+BETAS = {"zero": lambda r, T, h: np.zeros((T, h)), "one": lambda r, T, h: np.ones((T, h)),
+         "mixed": lambda r, T, h: (r.random((T, h)) < 0.5).astype(float)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", list(GATES))
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+@pytest.mark.parametrize("cut", [0, 64])
+def test_chunk_gates(lib, gate, dtype, cut):
+    Batch([130, 65, 3], hk=1, hv=2, dtype=dtype, gate=GATES[gate], seed=4).check(lib, cut=cut)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("beta", list(BETAS))
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+def test_chunk_betas(lib, beta, dtype):
+    Batch([130, 65, 3], hk=1, hv=2, dk=128, dtype=dtype, beta=BETAS[beta], seed=4).check(lib)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+@pytest.mark.parametrize("key_scale", [2.0 ** -30, 2.0 ** -12, 1.0])
+def test_chunk_key_magnitudes(lib, dtype, key_scale):
+    """Keys far below 1 without normalisation; with it, far above and below (any size normalises away)."""
+    Batch([100], dtype=dtype, l2norm=False, key_scale=key_scale, seed=8).check(lib)
+    Batch([100], dtype=dtype, l2norm=True, key_scale=1e6 * key_scale, seed=8).check(lib)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+def test_repeated_and_zero_keys(lib, dtype):
+    """All keys equal (the most ill-conditioned chunk of unit keys), then all keys zero."""
+    b = Batch([130], dtype=dtype, gate=GATES["none"], beta=BETAS["one"], seed=5)
+    for value in (0.7, 0.0):
+        b.k[1][:, :b.hk * b.dk] = value
+        b.host[1][:] = b.k[1][0, 0].double().item()
+        b.check(lib)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+@pytest.mark.parametrize("hk,hv,dk,dv", [(1, 1, 64, 16), (2, 2, 64, 64), (2, 8, 128, 128), (1, 3, 128, 144), (12, 12, 64, 64), (3, 3, 64, 256)])
+def test_step(lib, dtype, hk, hv, dk, dv):
+    for n in (1, 3, 40):
+        Batch([1] * n, hk=hk, hv=hv, dk=dk, dv=dv, dtype=dtype, l2norm=bool(n % 2), seed=n).check(lib, step=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", list(GATES))
+def test_step_gates(lib, gate):
+    Batch([1] * 9, hk=1, hv=2, dk=128, gate=GATES[gate], seed=4).check(lib, step=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+def test_rejected_requests(lib, step, dtype):
+    """A slot out of range: zero outputs for its rows, its inputs not used, the others as if it were absent."""
+    lens = [1, 1, 1] if step else [40, 70, 5]
+    b = Batch(lens, dtype=dtype, n_slots=6, slots=[4, NONE, 0], fresh=[0, 1, 0], seed=2)
+    rows = slice(int(b.cu[1]), int(b.cu[2]))
+    for x in (b.q, b.k, b.v, b.g, b.b):
+        x[1][rows] = float("nan")
+    out, st = b.check(lib, step=step)
+    assert b.word == 1 and (out[rows] == 0).all()
+    b.slots[1] = 6                                   # the first slot past the pool
+    b.check(lib, step=step)
+    assert b.word == 1
+    b.slots[1] = 2
+    b.lens, b.word = lens, None
+    b.fresh[1] = 1
+    out, st = b.run(lib, step=step)
+    assert b.word == 0 and np.isnan(out[rows]).all()  # NaN inputs stay in their own request
+    other = [i for i in range(b.T) if not rows.start <= i < rows.stop]
+    assert np.isfinite(out[other]).all() and np.isfinite(st[[4, 0]]).all()
+
+
+@pytest.mark.gpu
+def test_rejected_empty_request_is_no_error(lib):
+    b = Batch([3, 0], slots=[1, NONE], fresh=[0, 0], n_slots=3, seed=2)
+    b.check(lib)
+    assert b.word == 0
+
+
+@pytest.mark.gpu
+def test_empty_requests_and_no_requests(lib):
+    b = Batch([0, 0, 4], slots=[0, 1, 2], fresh=[0, 1, 0], n_slots=3)
+    _, st = b.check(lib)
+    assert np.array_equal(st[0], b.state[0].cpu().numpy()) and (st[1] == 0).all()
+    assert lib.delta_chunk(0, 0, 0, DTYPE_F32, 0, 0, 0, 0, 0, 0, 0, 1, 1, 64, 64, 64, 64, 64, 1, 64, 1.0, 0, 0, 0, 4096, 0, 0, 0, 0) == \
+        BackendResult.OK
+    assert lib.delta_step(0, 0, 0, DTYPE_F32, 0, 0, 0, 0, 0, 1, 1, 64, 64, 64, 64, 64, 1, 64, 1.0, 0, 0, 0, 4096, 0) == BackendResult.OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cut", [0, 64])
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+def test_same_bits_again_and_without_neighbours(lib, dtype, cut):
+    b = Batch([130, 77], dtype=dtype, hk=1, hv=2, seed=6)
+    o1, s1 = b.run(lib, cut=cut)
+    o2, s2 = b.run(lib, cut=cut)
+    assert np.array_equal(o1, o2) and np.array_equal(s1, s2)
+    alone = Batch([130, 77], dtype=dtype, hk=1, hv=2, seed=6)
+    alone.n, alone.lens, alone.T, alone.cu = 1, [130], 130, alone.cu[:2]
+    alone.slots, alone.fresh = alone.slots[:1], alone.fresh[:1]
+    alone.rows = 130
+    o3, s3 = alone.run(lib)
+    o4, s4 = b.run(lib)
+    assert np.array_equal(o3, o4[:130]) and np.array_equal(s3[b.slots[0]], s4[b.slots[0]])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+def test_prefill_then_steps(lib, dtype):
+    """A window's first tokens by delta_chunk, the rest one by one: the whole window's answer."""
+    whole = Batch([75], dtype=dtype, hk=1, hv=2, dk=128, fresh=[1], seed=12)
+    want, wst = whole.reference()
+    import torch
+    state = whole.state.clone()
+    part = Batch([75], dtype=dtype, hk=1, hv=2, dk=128, fresh=[1], seed=12)
+    part.lens, part.T, part.cu, part.rows = [70], 70, np.array([0, 70], np.uint32), 70
+    out, _ = part.run(lib, state=state)
+    outs = [out]
+    for t in range(70, 75):
+        one = Batch([75], dtype=dtype, hk=1, hv=2, dk=128, fresh=[0], seed=12)
+        for name in ("q", "k", "v", "g", "b"):
+            flat, view, ld = getattr(one, name)
+            setattr(one, name, (flat, view[t:t + 1], ld))
+        one.T, one.rows, one.lens = 1, 1, [1]
+        outs.append(one.run(lib, step=True, state=state)[0])
+    assert fits(np.concatenate(outs), want, dtype)
+    assert off_by(state.cpu().numpy()[whole.slots[0]], wst[whole.slots[0]]) <= F32
+
+
+@pytest.mark.gpu
+def test_on_a_stream_and_without_fresh(lib):
+    import torch
+    s = torch.cuda.Stream()
+    Batch([65, 10], seed=1).check(lib, stream=s.cuda_stream)
+    Batch([1, 1], seed=1).check(lib, step=True, stream=s.cuda_stream)
+    Batch([65, 10], seed=1, fresh=[0, 0]).check(lib, use_fresh=False)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(lib):
+    """A state pool and value rows that reach past 2^32 elements."""
+    import torch
+    b = Batch([1] * 6 + [70], hk=1, hv=1, dk=64, dv=64, dtype=DTYPE_BF16, n_slots=9, slots=[8, 0, 1, 2, 3, 4, 7], seed=3)
+    want, wst = b.reference()
+    stride = 1 << 29                               # floats: slot 8 starts at 2^32
+    state = torch.empty(8 * stride + 4096, device="cuda").as_strided((9, 1, 64, 64), (stride, 4096, 64, 1))
+    state.copy_(b.state)
+    rows, ld = b.T, 1 << 26                        # row 64 on starts past 2^32 elements
+    big = torch.empty((rows - 1) * ld + 64, dtype=torch.bfloat16, device="cuda")
+    view = big.as_strided((rows, 64), (ld, 1))
+    view.copy_(b.v[1][:, :64])
+    b.v = (big, view, ld)
+    out, _ = b.run(lib, state=state)
+    assert fits(out, want, DTYPE_BF16)
+    for s in b.slots:
+        assert off_by(state[int(s)].cpu().numpy(), wst[s]) <= F32
+
+
+def test_delta_refusals(lib):
+    """Host checks only: nothing reaches a device."""
+    head = dict(d_q=256, d_k=256, d_v=256, dtype=0, d_log_decay=256, d_beta=256)
+    tail = dict(d_slots=256, d_fresh=0, n_qk_heads=2, n_v_heads=4, d_key=64, d_value=64, ld_q=128, ld_k=128, ld_v=256, ld_gate=4,
+                ld_out=256, scale=1.0, l2norm=0, d_state=256, n_slots=4, slot_stride=4 * 64 * 64, d_out=256)
+    step = dict(head, n_streams=3, **tail)
+    chunk = dict(head, n_tokens=9, n_requests=3, d_cu=256, d_blocks=0, block=0, max_blocks=0, **tail)
+    changes = [dict(dtype=2), dict(dtype=-1), dict(n_qk_heads=0), dict(n_v_heads=0), dict(n_qk_heads=3), dict(d_key=32), dict(d_key=96),
+               dict(d_value=8), dict(d_value=40), dict(d_value=272, ld_v=2000, ld_out=2000, slot_stride=1 << 20), dict(ld_q=127),
+               dict(ld_k=127), dict(ld_v=255), dict(ld_gate=3), dict(ld_out=255), dict(slot_stride=4 * 64 * 64 - 4),
+               dict(slot_stride=4 * 64 * 64 + 2), dict(d_q=0), dict(d_k=0), dict(d_v=0), dict(d_log_decay=0), dict(d_beta=0),
+               dict(d_slots=0), dict(d_state=0), dict(d_state=264), dict(d_out=0), dict(d_out=258), dict(d_q=257), dict(d_log_decay=258),
+               dict(scale=float("nan"))]
+    for change in changes:
+        for fn, args, n in ((lib.delta_step, step, "n_streams"), (lib.delta_chunk, chunk, "n_requests")):
+            assert fn(**{**args, **change}) == BackendResult.INVALID_ARGUMENT, (n, change)
+            assert "delta_" in lib.last_error()
+    for change in [dict(n_requests=4097), dict(d_cu=0), dict(d_blocks=256, block=0, max_blocks=4), dict(d_blocks=256, block=100, max_blocks=4),
+                   dict(d_blocks=256, block=64, max_blocks=2), dict(d_work=8, work_bytes=1 << 20)]:
+        assert lib.delta_chunk(**{**chunk, **change}) == BackendResult.INVALID_ARGUMENT, change
+    assert lib.delta_step(**{**step, "n_streams": 4097}) == BackendResult.INVALID_ARGUMENT
+    assert lib.delta_work_bytes(10, 2, 64, 64) <= lib.delta_work_bytes(100, 2, 64, 64)

@@ -1,0 +1,144 @@
+"""plan_requests against a plain Python plan: whole numbers, equal everywhere."""
+import numpy as np
+import pytest
+
+from redukt_b200 import build as B
+from redukt_b200.plugin import BackendResult, PluginLibrary
+
+NONE = 0xFFFFFFFF
+
+
+@pytest.fixture(scope="module")
+def lib():
+    B.build()
+    return PluginLibrary()
+
+
+def plan(lengths, want, used, block, max_tokens, max_blocks):
+    """The rules of include/redukt_gpu.h, one request after the other."""
+    n, n_slots = len(lengths), len(used)
+    cu, base = [0], [0]
+    owner = {}
+    for i, w in enumerate(want):
+        if w < n_slots:
+            owner.setdefault(w, i)
+    free = [s for s in range(n_slots) if not used[s] and s not in owner]
+    slots, fresh, total, bad = [], [], 0, False
+    for i in range(n):
+        total += int(lengths[i])
+        fits = total <= max_tokens
+        cu.append(min(total, max_tokens))
+        base.append(base[-1] + -(-(cu[-1] - cu[-2]) // block))
+        slot, new = NONE, 0
+        if want[i] == NONE:
+            if lengths[i] > 0 and fits and free:
+                slot, new = free.pop(0), 1
+        elif owner.get(want[i]) == i and fits:
+            slot = int(want[i])
+        bad |= slot == NONE and (lengths[i] > 0 or want[i] != NONE)
+        slots.append(slot)
+        fresh.append(new)
+    used_out = [1 if used[s] or s in owner else 0 for s in range(n_slots)]
+    for s, f in zip(slots, fresh):
+        if f:
+            used_out[s] = 1
+    token_slot, token_pos = [NONE] * max_tokens, [NONE] * max_tokens
+    blocks = [[NONE, NONE]] * max_blocks
+    for i in range(n):
+        for t in range(cu[i], cu[i + 1]):
+            token_slot[t], token_pos[t] = slots[i], t - cu[i]
+        for b in range(base[i], base[i + 1]):
+            blocks[b] = [i, b - base[i]]
+    return dict(cu=cu, slots=slots, fresh=fresh, used_out=used_out, token_slot=token_slot, token_pos=token_pos,
+                block_base=base, blocks=blocks), bad
+
+
+def run(lib, lengths, want, used, block, max_tokens, max_blocks, off=0, stream=0):
+    import torch
+
+    def dev(x, dtype):
+        return torch.from_numpy(np.asarray(x, np.uint32 if dtype is torch.int32 else np.uint8).view(
+            np.int32 if dtype is torch.int32 else np.uint8).copy()).cuda()
+
+    def out(n, dtype=torch.int32):   # one guard element on each side, `off` shifts the alignment
+        return torch.full((n + 2 + off,), 77, dtype=dtype, device="cuda")
+
+    n, n_slots = len(lengths), len(used)
+    a = [dev(lengths, torch.int32), dev(want, torch.int32), dev(used, torch.uint8)]
+    sizes = dict(cu=n + 1, slots=n, fresh=n, used_out=n_slots, token_slot=max_tokens, token_pos=max_tokens,
+                 block_base=n + 1, blocks=2 * max_blocks)
+    bufs = {k: out(s, torch.uint8 if k == "used_out" else torch.int32) for k, s in sizes.items()}
+    ptr = {k: b[1 + off:].data_ptr() for k, b in bufs.items()}
+    torch.cuda.synchronize()
+    rc = lib.plan_requests(a[0].data_ptr(), a[1].data_ptr(), n, a[2].data_ptr(), n_slots, block, max_tokens, max_blocks,
+                           ptr["cu"], ptr["slots"], ptr["fresh"], ptr["used_out"], ptr["token_slot"], ptr["token_pos"],
+                           ptr["block_base"], ptr["blocks"], stream)
+    assert rc == BackendResult.OK, lib.last_error()
+    word = lib.ops_error()
+    got = {}
+    for k, b in bufs.items():
+        h = b.cpu().numpy()
+        assert (h[:1 + off] == 77).all() and h[1 + off + sizes[k]] == 77, k
+        got[k] = h[1 + off:1 + off + sizes[k]].view(np.uint8 if k == "used_out" else np.uint32)
+    return got, word
+
+
+def check(lib, lengths, want, used, block, max_tokens=None, max_blocks=None, **kw):
+    max_tokens = sum(int(x) for x in lengths) if max_tokens is None else max_tokens
+    max_blocks = max_tokens // block + len(lengths) if max_blocks is None else max_blocks
+    ref, bad = plan(lengths, want, used, block, max_tokens, max_blocks)
+    got, word = run(lib, lengths, want, used, block, max_tokens, max_blocks, **kw)
+    for k, r in ref.items():
+        assert np.array_equal(got[k].astype(np.int64), np.asarray(r, np.int64).reshape(-1)), k
+    assert word == (1 if bad else 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,n_slots,mean,block", [(1, 1, 1, 64), (1, 8, 300, 64), (2, 3, 5, 1), (7, 16, 40, 64),
+                                                  (33, 20, 3, 7), (100, 300, 90, 128), (1023, 1024, 9, 64),
+                                                  (1025, 4096, 20, 256), (4095, 4095, 6, 64), (4096, 4096, 11, 1000)])
+@pytest.mark.parametrize("seed", [0, 1])
+def test_plan_random(lib, n, n_slots, mean, block, seed):
+    r = np.random.default_rng(seed * 7919 + n)
+    lengths = np.where(r.random(n) < 0.2, 0, r.integers(0, 2 * mean + 1, n))
+    want = np.where(r.random(n) < 0.4, r.integers(0, n_slots, n), NONE)
+    used = (r.random(n_slots) < 0.5).astype(np.uint8) * r.integers(1, 256, n_slots)
+    check(lib, lengths, want, used, block, off=seed)
+
+
+@pytest.mark.gpu
+def test_plan_edges(lib):
+    z = [0] * 8
+    check(lib, [], [], z, 64, max_tokens=5)                                     # no requests: everything is padding
+    check(lib, [], [], [], 64)
+    check(lib, [0, 0, 0], [NONE, 3, NONE], z, 64, max_tokens=2)                 # nobody has tokens, one keeps its slot
+    check(lib, [3, 4], [NONE, NONE], [], 64)                                    # no slots at all: both rejected
+    check(lib, [1] * 12, [NONE] * 12, z, 64)                                    # the pool runs out after eight
+    check(lib, [2, 2, 2], [5, 5, 5], z, 64)                                     # three ask for one slot: the first has it
+    check(lib, [2, 2, 2], [8, NONE - 1, 0], z, 64)                              # out of range
+    check(lib, [0, 3], [2, 2], z, 64)                                           # an empty request still owns its slot
+    check(lib, [5, 5, 0, 5], [NONE, NONE, 1, NONE], z, 4, max_tokens=9)         # the second ends above max_tokens
+    check(lib, [5, 5, 5], [NONE, 0, NONE], z, 4, max_tokens=12)                 # the named slot of one that fits, the last cut
+    check(lib, [NONE, NONE, 3], [NONE, 1, NONE], z, 64, max_tokens=100)         # sums past 32 bits
+    check(lib, [7, 9], [NONE, NONE], [1] * 8, 64, max_tokens=40, max_blocks=9)  # padding past the last token and block
+
+
+@pytest.mark.gpu
+def test_plan_on_a_stream_many_tokens(lib):
+    import torch
+    s = torch.cuda.Stream()
+    r = np.random.default_rng(5)
+    lengths = r.integers(0, 1500, 700)
+    check(lib, lengths, np.full(700, NONE), np.zeros(4096, np.uint8), 64, stream=s.cuda_stream)
+
+
+def test_plan_refusals(lib):
+    """Host checks only: nothing reaches a device."""
+    ok = dict(d_lengths=64, d_want=64, n=2, d_used=64, n_slots=4, block=64, max_tokens=10, max_blocks=2, d_cu=64, d_slots=64,
+              d_fresh=64, d_used_out=128, d_token_slot=64, d_token_pos=64, d_block_base=64, d_blocks=64)
+    bad = [dict(n=4097, max_blocks=5000), dict(n_slots=4097), dict(block=0), dict(max_blocks=1), dict(d_lengths=0), dict(d_want=0),
+           dict(d_used=0), dict(d_cu=0), dict(d_slots=0), dict(d_fresh=0), dict(d_used_out=0), dict(d_used_out=64),
+           dict(d_token_slot=0), dict(d_token_pos=0), dict(d_block_base=0), dict(d_blocks=0), dict(max_tokens=NONE)]
+    for change in bad:
+        assert lib.plan_requests(**{**ok, **change}) == BackendResult.INVALID_ARGUMENT, change
+        assert "plan_requests" in lib.last_error()

@@ -1,0 +1,287 @@
+"""quantize_tokens, w8a8_matmul, w8a8_linear: the integer sum is exact and every other step is one
+correctly rounded f32 operation, so outputs equal the plain computation's bit for bit."""
+import numpy as np
+import pytest
+
+from redukt_b200 import build as B
+from redukt_b200.plugin import DTYPE_BF16, DTYPE_F32, BackendResult, PluginLibrary
+
+
+@pytest.fixture(scope="module")
+def lib():
+    B.build()
+    return PluginLibrary()
+
+
+def quantize(x):
+    """quantize_tokens' recipe (include/redukt_gpu.h) on f32 rows, in numpy f32 steps."""
+    x = np.asarray(x, np.float32)
+    with np.errstate(all="ignore"):
+        mag = np.where(np.isnan(x), np.float32(0), np.abs(x))
+        top = mag.max(1).astype(np.float32)
+        scale = np.where(top > 0, top * (np.float32(1) / np.float32(127)), np.float32(1)).astype(np.float32)
+        t = x * (np.float32(1) / scale)[:, None]
+        r = np.copysign(np.floor(np.abs(t.astype(np.float64)) + 0.5), t)  # half away from zero, exact in f64
+        q = np.where(np.isnan(t), 0.0, np.clip(r, -127, 127)).astype(np.int8)
+    return q, scale
+
+
+def product(a, a_scale, w, w_scale):
+    acc = a.astype(np.float64) @ w.astype(np.float64).T          # below 2^53: exact
+    with np.errstate(all="ignore"):
+        return acc.astype(np.float32) * (w_scale[None, :].astype(np.float32) * a_scale[:, None].astype(np.float32))
+
+
+def same_bits(got, want):
+    g, w = np.ascontiguousarray(got), np.ascontiguousarray(want)
+    both = np.isnan(g) & np.isnan(w)
+    return bool(np.all((g.view(np.uint32) == w.view(np.uint32)) | both))
+
+
+def bf16(x):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(x, np.float32)).to(torch.bfloat16).float().numpy()
+
+
+def padded(q, extra=0):
+    """int8 rows on a device at a stride that is a multiple of 16, the padding full of 99."""
+    import torch
+    m, k = q.shape
+    ld = -(-k // 16) * 16 + extra
+    h = np.full((m, ld), 99, np.int8)
+    h[:, :k] = q
+    return torch.from_numpy(h).cuda(), ld
+
+
+def out_buffer(m, n, dtype, ld):
+    import torch
+    return torch.full((m, ld), -7.0, dtype=torch.bfloat16 if dtype == DTYPE_BF16 else torch.float32, device="cuda")
+
+
+def result(buf, n):
+    h = buf.float().cpu().numpy()
+    assert (h[:, n:] == -7.0).all()   # between the row's end and its stride nothing is written
+    return h[:, :n]
+
+
+def workspace(lib, m, n, k):
+    import torch
+    return torch.full((max(256, lib.w8a8_work_bytes(m, n, k)),), 0x5A, dtype=torch.uint8, device="cuda")
+
+
+def check_matmul(lib, m, n, k, dtype, extra=0, ld_extra=0, seed=0, work=True, lo=-128):
+    import torch
+    r = np.random.default_rng(seed + 31 * m + 7 * n + k)
+    a, w = r.integers(lo, 128, (m, k)).astype(np.int8), r.integers(lo, 128, (n, k)).astype(np.int8)
+    sa, sw = (r.random(m) + 0.5).astype(np.float32), (r.random(n) + 0.1).astype(np.float32)
+    da, lda = padded(a, extra)
+    dw, ldw = padded(w, extra)
+    dsa, dsw = torch.from_numpy(sa).cuda(), torch.from_numpy(sw).cuda()
+    out = out_buffer(m, n, dtype, n + ld_extra)
+    ws = workspace(lib, m, n, k)
+    rc = lib.w8a8_matmul(da.data_ptr(), lda, dsa.data_ptr(), m, dw.data_ptr(), ldw, dsw.data_ptr(), n, k, out.data_ptr(), dtype,
+                         n + ld_extra, ws.data_ptr() if work else 0, ws.numel() if work else 0)
+    assert rc == BackendResult.OK, lib.last_error()
+    assert lib.ops_error() == 0
+    want = product(a, sa, w, sw)
+    assert same_bits(result(out, n), bf16(want) if dtype == DTYPE_BF16 else want)
+
+
+def check_linear(lib, x, w, sw, dtype, out_dtype, ld_x=None, off=0, stream=0):
+    import torch
+    m, k = x.shape
+    n = w.shape[0]
+    ld_x = ld_x or k
+    t = torch.bfloat16 if dtype == DTYPE_BF16 else torch.float32
+    flat = torch.full((m * ld_x + off,), float("nan"), dtype=t, device="cuda")
+    rows = flat[off:].view(m, ld_x)
+    rows[:, :k] = torch.from_numpy(np.ascontiguousarray(x, np.float32)).cuda().to(t)
+    xin = rows[:, :k].float().cpu().numpy()
+    dw, ldw = padded(w)
+    dsw = torch.from_numpy(sw).cuda()
+    out = out_buffer(m, n, out_dtype, n + 3)
+    ws = workspace(lib, m, n, k)
+    torch.cuda.synchronize()
+    rc = lib.w8a8_linear(rows.data_ptr(), dtype, m, k, ld_x, dw.data_ptr(), ldw, dsw.data_ptr(), n, out.data_ptr(), out_dtype, n + 3,
+                         ws.data_ptr(), ws.numel(), stream)
+    assert rc == BackendResult.OK, lib.last_error()
+    assert lib.ops_error() == 0
+    q, s = quantize(xin)
+    want = product(q, s, w, sw)
+    assert same_bits(result(out, n), bf16(want) if out_dtype == DTYPE_BF16 else want)
+
+
+def random_linear(lib, m, n, k, dtype, out_dtype, **kw):
+    r = np.random.default_rng(m + 3 * n + 5 * k)
+    x = r.standard_normal((m, k)) * np.exp(r.uniform(-6, 6, (m, 1)))
+    x[r.random((m, k)) < 0.01] *= 30
+    x[m // 2] = 0 if m > 2 else x[m // 2]
+    check_linear(lib, x, r.integers(-127, 128, (n, k)).astype(np.int8), (r.random(n) + 0.1).astype(np.float32), dtype, out_dtype, **kw)
+
+
+SIZES = [(1, 1, 1), (1, 5, 17), (2, 64, 64), (3, 100, 15), (1, 257, 768), (7, 130, 200), (8, 1000, 1000), (15, 33, 129),
+         (16, 768, 768), (17, 128, 31), (32, 2304, 768), (33, 96, 4096), (64, 64, 128), (65, 513, 300), (100, 63, 2048),
+         (128, 256, 512), (129, 257, 127), (200, 1111, 1000), (256, 512, 64), (300, 300, 300), (777, 130, 1000), (1030, 384, 257)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+def test_matmul_sizes(lib, m, n, k, dtype):
+    check_matmul(lib, m, n, k, dtype, extra=16 * (m % 3), ld_extra=(m + n) % 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 300, 5000), (40, 70, 768), (513, 700, 1024)])
+def test_matmul_without_workspace(lib, m, n, k):
+    check_matmul(lib, m, n, k, DTYPE_F32, work=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 130])
+def test_matmul_largest_sum(lib, m):
+    """k = 131071 with every product 2^14: the largest sum, 2^31 - 2^14."""
+    import torch
+    k, n = 131071, 130
+    a, w = np.full((m, k), -128, np.int8), np.full((n, k), -128, np.int8)
+    one = np.ones(max(m, n), np.float32)
+    da, lda = padded(a)
+    dw, ldw = padded(w)
+    ones = torch.from_numpy(one).cuda()
+    out = out_buffer(m, n, DTYPE_F32, n)
+    assert lib.w8a8_matmul(da.data_ptr(), lda, ones.data_ptr(), m, dw.data_ptr(), ldw, ones.data_ptr(), n, k, out.data_ptr(),
+                           DTYPE_F32, n) == BackendResult.OK
+    assert lib.ops_error() == 0
+    assert same_bits(result(out, n), product(a, one[:m], w, one[:n]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_linear_sizes(lib, m, n, k):
+    random_linear(lib, m, n, k, (m + n) % 2, k % 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+@pytest.mark.parametrize("m", [1, 5, 40, 150])
+def test_linear_strides_and_alignment(lib, dtype, m):
+    random_linear(lib, m, 70, 96, dtype, DTYPE_F32, ld_x=101)
+    random_linear(lib, m, 70, 96, dtype, DTYPE_F32, ld_x=104, off=1)
+    random_linear(lib, m, 70, 99, dtype, DTYPE_BF16, ld_x=112, off=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [12, 140])
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+def test_linear_special_values(lib, m, dtype):
+    r = np.random.default_rng(3)
+    k, n = 200, 96
+    x = r.standard_normal((m, k))
+    x[0, 3] = np.nan
+    x[1, :] = np.nan
+    x[2, 5], x[2, 6] = np.inf, -np.inf
+    x[3, :] = 0.0
+    x[4, :] *= 1e-39      # f32 subnormals: the reciprocal of the scale overflows
+    x[5, :] = np.tile([127.0, 0.5, -0.5, 1.5, -1.5, 2.5, 126.5, -126.5], k // 8)   # ties, scale 1
+    x[6, :] = 3e38
+    x[7, :] = -0.0
+    w, sw = r.integers(-127, 128, (n, k)).astype(np.int8), (r.random(n) + 0.1).astype(np.float32)
+    check_linear(lib, x, w, sw, dtype, DTYPE_F32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+@pytest.mark.parametrize("m,k,ld_x,ld_q,off", [(1, 1, 1, 1, 0), (5, 768, 768, 768, 0), (3, 1001, 1003, 1009, 1), (300, 64, 64, 80, 0),
+                                               (2, 20000, 20000, 20000, 0), (4, 131071, 131071, 131072, 0)])
+def test_quantize_tokens(lib, dtype, m, k, ld_x, ld_q, off):
+    import torch
+    t = torch.bfloat16 if dtype == DTYPE_BF16 else torch.float32
+    x = torch.randn(m * ld_x + off, device="cuda", generator=torch.Generator("cuda").manual_seed(k)).to(t)
+    q = torch.full((m, ld_q), 99, dtype=torch.int8, device="cuda")
+    s = torch.empty(m, device="cuda")
+    assert lib.quantize_tokens(x[off:].data_ptr(), dtype, m, k, ld_x, q.data_ptr(), ld_q, s.data_ptr()) == BackendResult.OK
+    torch.cuda.synchronize()
+    wq, ws = quantize(x[off:].view(m, ld_x)[:, :k].float().cpu().numpy())
+    assert np.array_equal(q.cpu().numpy()[:, :k], wq) and (q.cpu().numpy()[:, k:] == 99).all()
+    assert np.array_equal(s.cpu().numpy(), ws)
+
+
+@pytest.mark.gpu
+def test_linear_on_a_stream_and_repeatable(lib):
+    import torch
+    s = torch.cuda.Stream()
+    for m in (1, 20, 260):
+        random_linear(lib, m, 700, 1500, DTYPE_BF16, DTYPE_F32, stream=s.cuda_stream)
+
+
+@pytest.mark.gpu
+def test_a_row_has_the_same_bits_in_every_batch(lib):
+    """One token alone, and the same token among others, through whatever kernels those sizes take."""
+    import torch
+    r = np.random.default_rng(11)
+    n, k = 520, 960
+    a = r.integers(-127, 128, (600, k)).astype(np.int8)
+    w, ldw = padded(r.integers(-127, 128, (n, k)).astype(np.int8))
+    sw = torch.rand(n, device="cuda")
+    sa = torch.rand(600, device="cuda")
+    da, lda = padded(a)
+    rows = {}
+    for m in (1, 4, 16, 40, 130, 600):
+        out = out_buffer(m, n, DTYPE_F32, n)
+        ws = workspace(lib, m, n, k)
+        assert lib.w8a8_matmul(da.data_ptr(), lda, sa.data_ptr(), m, w.data_ptr(), ldw, sw.data_ptr(), n, k, out.data_ptr(), DTYPE_F32,
+                               n, ws.data_ptr(), ws.numel()) == BackendResult.OK
+        rows[m] = result(out, n)[0]
+    assert lib.ops_error() == 0
+    assert all(same_bits(v, rows[1]) for v in rows.values())
+
+
+@pytest.mark.gpu
+def test_output_offsets_past_32_bits(lib):
+    """Rows 2^31 elements apart: the last ones start past 2^32 elements (8.6 GB of bf16, unwritten elsewhere)."""
+    import torch
+    m, n, k, ld = 3, 64, 64, 1 << 31
+    r = np.random.default_rng(2)
+    a, w = r.integers(-127, 128, (m, k)).astype(np.int8), r.integers(-127, 128, (n, k)).astype(np.int8)
+    one = np.ones(64, np.float32)
+    da, lda = padded(a)
+    dw, ldw = padded(w)
+    ones = torch.from_numpy(one).cuda()
+    out = torch.empty(2 * ld + n, dtype=torch.bfloat16, device="cuda")
+    assert lib.w8a8_matmul(da.data_ptr(), lda, ones.data_ptr(), m, dw.data_ptr(), ldw, ones.data_ptr(), n, k, out.data_ptr(), DTYPE_BF16,
+                           ld) == BackendResult.OK
+    got = np.stack([out[i * ld:i * ld + n].float().cpu().numpy() for i in range(m)])
+    assert lib.ops_error() == 0
+    assert same_bits(got, bf16(product(a, one[:m], w, one)))
+
+
+def test_w8a8_refusals(lib):
+    """Host checks only: nothing reaches a device."""
+    bad = BackendResult.INVALID_ARGUMENT
+    mm = dict(d_a=256, ld_a=64, d_a_scale=256, n_tokens=4, d_w=256, ld_w=64, d_w_scale=256, n_out=8, k=60, d_out=256, out_dtype=0, ld_out=8)
+    for change in [dict(k=0), dict(k=131072, ld_a=131072, ld_w=131072), dict(ld_a=48), dict(ld_a=72), dict(ld_w=48), dict(ld_w=72),
+                   dict(d_a=264), dict(d_w=264), dict(ld_out=7), dict(out_dtype=2), dict(out_dtype=-1), dict(d_a=0), dict(d_w=0),
+                   dict(d_a_scale=0), dict(d_w_scale=0), dict(d_out=0), dict(d_out=258), dict(n_tokens=1 << 31)]:
+        assert lib.w8a8_matmul(**{**mm, **change}) == bad, change
+        assert "w8a8_matmul" in lib.last_error()
+    need = lib.w8a8_work_bytes(4, 8, 60)
+    li = dict(d_x=256, dtype=0, n_tokens=4, k=60, ld_x=60, d_w=256, ld_w=64, d_w_scale=256, n_out=8, d_out=256, out_dtype=0, ld_out=8,
+              d_work=256, work_bytes=need)
+    for change in [dict(dtype=3), dict(ld_x=59), dict(d_x=0), dict(d_x=257), dict(d_work=0), dict(d_work=16), dict(work_bytes=need - 1),
+                   dict(k=0), dict(ld_w=56), dict(out_dtype=5), dict(ld_out=3)]:
+        assert lib.w8a8_linear(**{**li, **change}) == bad, change
+        assert "w8a8_linear" in lib.last_error()
+    qt = dict(d_x=256, dtype=1, n_tokens=4, k=60, ld_x=60, d_q=256, ld_q=60, d_scale=256)
+    for change in [dict(dtype=2), dict(k=0), dict(k=131072, ld_x=131072, ld_q=131072), dict(ld_x=59), dict(ld_q=59), dict(d_x=0), dict(d_q=0),
+                   dict(d_scale=0), dict(d_x=255), dict(d_scale=254)]:
+        assert lib.quantize_tokens(**{**qt, **change}) == bad, change
+        assert "quantize_tokens" in lib.last_error()
+    # nothing to do is no error, with no device touched
+    assert lib.w8a8_matmul(**{**mm, "n_tokens": 0}) == BackendResult.OK
+    assert lib.w8a8_linear(**{**li, "n_out": 0}) == BackendResult.OK
+    assert lib.quantize_tokens(**{**qt, "n_tokens": 0}) == BackendResult.OK
+
+
+def test_w8a8_work_bytes_grow_with_the_batch(lib):
+    sizes = [lib.w8a8_work_bytes(m, 4096, 1000) for m in (1, 100, 10000)]
+    assert sizes == sorted(sizes) and sizes[2] >= 10000 * 1004
