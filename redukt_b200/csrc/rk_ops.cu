@@ -2,6 +2,7 @@
 // They need no model loaded, allocate nothing and keep nothing between calls; every launch goes
 // to the caller's stream.
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <cmath>
@@ -44,8 +45,14 @@ struct Device {
     bool ready = false;
     uint32_t* err = nullptr;
     int sms = 0;
+    PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
 };
 Device g_device[kMaxDevices];
+
+template <int BN, class T>
+cudaError_t set_smem() {
+    return cudaFuncSetAttribute(rk::w8::k_w8a8_tc<BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rk::w8::tc_smem<BN>());
+}
 
 // The current device's facts; the first call on a device looks them up and sets the kernels'
 // shared-memory limits.
@@ -61,6 +68,20 @@ int32_t device(Device** out) {
         d.err = static_cast<uint32_t*>(p);
         OP_CK(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
         OP_CK(cudaFuncSetAttribute(rk::plan::k_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::plan::Smem)));
+        OP_CK((set_smem<256, float>()));
+        OP_CK((set_smem<256, __nv_bfloat16>()));
+        OP_CK((set_smem<128, float>()));
+        OP_CK((set_smem<128, __nv_bfloat16>()));
+        OP_CK((set_smem<64, float>()));
+        OP_CK((set_smem<64, __nv_bfloat16>()));
+        cudaDriverEntryPointQueryResult found;
+        void* fn = nullptr;
+        OP_CK(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+        if (found != cudaDriverEntryPointSuccess || !fn) {
+            set_err("the driver has no cuTensorMapEncodeTiled");
+            return BACKEND_FORWARD_FAILED;
+        }
+        d.encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
         d.ready = true;
     }
     *out = &d;
@@ -118,20 +139,84 @@ int32_t w8_check(const char* what, uint32_t n_tokens, uint32_t n_out, uint32_t k
 
 int32_t quantize(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q, uint64_t ld_q,
                  float* d_scale, cudaStream_t st) {
+    using namespace rk::w8;
     if (dtype == REDUKT_DTYPE_F32)
-        rk::w8::k_quant_tokens<float><<<n_tokens, 256, 0, st>>>((const float*)d_x, k, ld_x, d_q, ld_q, d_scale);
+        k_quant_tokens<float><<<n_tokens, kQuantThreads, 0, st>>>((const float*)d_x, k, ld_x, d_q, ld_q, d_scale);
     else
-        rk::w8::k_quant_tokens<__nv_bfloat16><<<n_tokens, 256, 0, st>>>((const __nv_bfloat16*)d_x, k, ld_x, d_q, ld_q, d_scale);
+        k_quant_tokens<__nv_bfloat16><<<n_tokens, kQuantThreads, 0, st>>>((const __nv_bfloat16*)d_x, k, ld_x, d_q, ld_q, d_scale);
     OP_CK(cudaGetLastError());
     return BACKEND_OK;
 }
 
-int32_t matmul(const rk::w8::Args& a, int32_t out_dtype, cudaStream_t st) {
-    const dim3 grid((unsigned)ceil_div(a.n, 64), (unsigned)ceil_div(a.m, 64));
-    if (out_dtype == REDUKT_DTYPE_F32) rk::w8::k_w8a8_dp4a<float><<<grid, 256, 0, st>>>(a);
-    else rk::w8::k_w8a8_dp4a<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-    OP_CK(cudaGetLastError());
+// A 2-D tensor map over rows of `width` elements, boxes of 128 bytes x box_rows in the 128-byte swizzle.
+int32_t tensor_map(CUtensorMap* map, const Device& d, CUtensorMapDataType type, size_t elem, const void* base, uint64_t width,
+                   uint64_t rows, uint64_t ld, uint32_t box_rows) {
+    const cuuint64_t dims[2] = {width, rows}, strides[1] = {ld * elem};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / elem), box_rows}, one[2] = {1, 1};
+    const CUresult r = d.encode(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_err("cuTensorMapEncodeTiled failed (%d) for %llu x %llu at stride %llu", (int)r, (unsigned long long)rows,
+                (unsigned long long)width, (unsigned long long)ld);
+        return BACKEND_FORWARD_FAILED;
+    }
     return BACKEND_OK;
+}
+
+template <int BN, class T>
+int32_t launch_tc(const Device& d, const rk::w8::Args& a, cudaStream_t st, bool after_quant) {
+    using namespace rk::w8;
+    CUtensorMap ma, mw, mo;
+    if (int32_t rc = tensor_map(&ma, d, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.a, a.k, a.m, a.ld_a, kTileM)) return rc;
+    if (int32_t rc = tensor_map(&mw, d, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.k, a.n, a.ld_w, BN)) return rc;
+    const bool tma_out = aligned(a.out, 16) && a.ld_o * sizeof(T) % 16 == 0;
+    if (tma_out) {
+        const CUtensorMapDataType t = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        if (int32_t rc = tensor_map(&mo, d, t, sizeof(T), a.out, a.n, a.m, a.ld_o, 32)) return rc;
+    } else {
+        mo = ma;   // never used
+    }
+    TcArgs g = {a.as, a.ws, a.out, a.ld_o, a.m, a.n, a.k, (uint32_t)ceil_div(a.m, kTileM), (uint32_t)ceil_div(a.n, BN), tma_out, d.err};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::min<uint64_t>((uint64_t)g.tiles_m * g.tiles_n, d.sms));
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = tc_smem<BN>();
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = after_quant ? 1 : 0;
+    OP_CK(cudaLaunchKernelEx(&cfg, k_w8a8_tc<BN, T>, ma, mw, mo, g));
+    return BACKEND_OK;
+}
+
+// Width of the tensor-core tile: the one whose waves over the SMs cost least, a tile of BN channels
+// taking about as long as BN + 32 (its fill and drain do not shrink with it).
+int tile_width(uint64_t m, uint64_t n, int sms) {
+    int best = 256;
+    uint64_t least = ~0ull;
+    for (int bn : {256, 128, 64}) {
+        const uint64_t waves = ceil_div(ceil_div(m, rk::w8::kTileM) * ceil_div(n, bn), sms), cost = waves * (bn + 32);
+        if (cost < least) {
+            least = cost;
+            best = bn;
+        }
+    }
+    return best;
+}
+
+template <class T>
+int32_t matmul_t(const Device& d, const rk::w8::Args& a, cudaStream_t st, bool after_quant) {
+    switch (tile_width(a.m, a.n, d.sms)) {
+        case 256: return launch_tc<256, T>(d, a, st, after_quant);
+        case 128: return launch_tc<128, T>(d, a, st, after_quant);
+        default: return launch_tc<64, T>(d, a, st, after_quant);
+    }
+}
+
+int32_t matmul(const Device& d, const rk::w8::Args& a, int32_t out_dtype, cudaStream_t st, bool after_quant) {
+    return out_dtype == REDUKT_DTYPE_F32 ? matmul_t<float>(d, a, st, after_quant) : matmul_t<__nv_bfloat16>(d, a, st, after_quant);
 }
 
 uint64_t quant_ld(uint32_t k) { return ceil_div(k, 16) * 16; }
@@ -266,7 +351,9 @@ int32_t redukt_b200_w8a8_matmul(const int8_t* d_a, uint64_t ld_a, const float* d
     OP_REQUIRE(d_a && d_a_scale, "w8a8_matmul: NULL argument");
     OP_REQUIRE(ld_a >= k && ld_a % 16 == 0 && aligned(d_a, 16) && aligned(d_a_scale, 4), "w8a8_matmul: int8 rows must start on 16 bytes and hold k values");
     rk::w8::Args a = {d_a, d_a_scale, d_w, d_w_scale, ld_a, ld_w, ld_out, n_tokens, n_out, k, d_out};
-    return matmul(a, out_dtype, stream_of(cuda_stream));
+    Device* d = nullptr;
+    if (int32_t rc = device(&d)) return rc;
+    return matmul(*d, a, out_dtype, stream_of(cuda_stream), false);
 }
 
 int32_t redukt_b200_w8a8_linear(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, const int8_t* d_w,
@@ -280,10 +367,12 @@ int32_t redukt_b200_w8a8_linear(const void* d_x, int32_t dtype, uint32_t n_token
                "w8a8_linear: the workspace needs %llu bytes on 256", (unsigned long long)redukt_b200_w8a8_work_bytes(n_tokens, n_out, k));
     int8_t* q = static_cast<int8_t*>(d_work);
     float* s = reinterpret_cast<float*>(q + ceil_div((uint64_t)n_tokens * quant_ld(k), 256) * 256);
+    Device* d = nullptr;
+    if (int32_t rc = device(&d)) return rc;
     const cudaStream_t st = stream_of(cuda_stream);
     if (int32_t rc = quantize(d_x, dtype, n_tokens, k, ld_x, q, quant_ld(k), s, st)) return rc;
     rk::w8::Args a = {q, s, d_w, d_w_scale, quant_ld(k), ld_w, ld_out, n_tokens, n_out, k, d_out};
-    return matmul(a, out_dtype, st);
+    return matmul(*d, a, out_dtype, st, true);
 }
 
 }  // extern "C"

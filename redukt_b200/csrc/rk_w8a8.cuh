@@ -5,10 +5,13 @@
 // Each f32 operation is correctly rounded and the sum is exact in int32, so every kernel here gives
 // the same bits.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+
+#include "rk_ptx.cuh"
 
 namespace rk {
 namespace w8 {
@@ -27,26 +30,84 @@ __device__ __forceinline__ int quant_one(float v, float inv) {
 __device__ __forceinline__ float row_scale(float amax) { return amax > 0.f ? __fmul_rn(amax, 1.f / 127.f) : 1.f; }
 
 // One block per token: the row's largest magnitude (exact in any order), then its 8-bit values.
-// The row's tail up to ld_q's multiple of 16 is not written.
+// Bound by the bytes of the row in and out: it is read once, as 16-byte vectors kept in registers
+// (up to kHold a thread; longer or unaligned rows are read again).
+constexpr int kQuantThreads = 128;
+constexpr int kHold = 8;
+
 template <class T>
-__global__ void __launch_bounds__(256) k_quant_tokens(const T* __restrict__ x, uint32_t k, uint64_t ld_x, int8_t* __restrict__ q,
-                                                      uint64_t ld_q, float* __restrict__ scale) {
-    __shared__ float part[8];
-    const uint64_t row = blockIdx.x;
-    const T* xr = x + row * ld_x;
-    float m = 0.f;
-    for (uint32_t i = threadIdx.x; i < k; i += blockDim.x) m = fmaxf(m, fabsf(to_f32(xr[i])));
+struct Vec {   // 16 bytes of activations
+    static constexpr int kN = 16 / sizeof(T);
+    uint4 raw;
+    __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(&raw)[i]); }
+};
+
+template <class T>
+__device__ __forceinline__ void put_quant(int8_t* q, const Vec<T>& v, float inv) {   // 8 (bf16) or 4 (f32) bytes
+    uint32_t w[Vec<T>::kN / 4];
+#pragma unroll
+    for (int i = 0; i < Vec<T>::kN; i++) {
+        const uint32_t b = (uint32_t)(quant_one(v.get(i), inv) & 255) << (8 * (i & 3));
+        w[i >> 2] = (i & 3) ? w[i >> 2] | b : b;
+    }
+    if constexpr (Vec<T>::kN == 8) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(q) = w[0];
+}
+
+__device__ __forceinline__ float block_max(float m, float* part) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
     __syncthreads();
     m = part[0];
 #pragma unroll
-    for (int i = 1; i < 8; i++) m = fmaxf(m, part[i]);
+    for (int i = 1; i < kQuantThreads / 32; i++) m = fmaxf(m, part[i]);
+    return m;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kQuantThreads) k_quant_tokens(const T* __restrict__ x, uint32_t k, uint64_t ld_x, int8_t* __restrict__ q,
+                                                                uint64_t ld_q, float* __restrict__ scale) {
+    __shared__ float part[kQuantThreads / 32];
+    tc::grid_trigger();   // a product launched after this kernel sets itself up meanwhile
+    constexpr int N = Vec<T>::kN;
+    const T* xr = x + blockIdx.x * ld_x;
+    int8_t* qr = q + blockIdx.x * ld_q;
+    const bool wide = ((reinterpret_cast<uintptr_t>(xr) & 15) | (reinterpret_cast<uintptr_t>(qr) & (N - 1))) == 0;
+    const uint32_t nv = wide ? k / N : 0;   // whole vectors; the rest one by one
+    float m = 0.f;
+    Vec<T> v[kHold];
+#pragma unroll
+    for (int i = 0; i < kHold; i++) {
+        const uint32_t j = threadIdx.x + i * kQuantThreads;
+        if (j < nv) {
+            v[i].raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
+#pragma unroll
+            for (int c = 0; c < N; c++) m = fmaxf(m, fabsf(v[i].get(c)));
+        }
+    }
+    for (uint32_t j = threadIdx.x + kHold * kQuantThreads; j < nv; j += kQuantThreads) {
+        Vec<T> u;
+        u.raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
+#pragma unroll
+        for (int c = 0; c < N; c++) m = fmaxf(m, fabsf(u.get(c)));
+    }
+    for (uint32_t c = nv * N + threadIdx.x; c < k; c += kQuantThreads) m = fmaxf(m, fabsf(to_f32(xr[c])));
+    m = block_max(m, part);
     const float s = row_scale(m);
     const float inv = __fdiv_rn(1.f, s);
-    for (uint32_t i = threadIdx.x; i < k; i += blockDim.x) q[row * ld_q + i] = (int8_t)quant_one(to_f32(xr[i]), inv);
-    if (threadIdx.x == 0) scale[row] = s;
+#pragma unroll
+    for (int i = 0; i < kHold; i++) {
+        const uint32_t j = threadIdx.x + i * kQuantThreads;
+        if (j < nv) put_quant(qr + (uint64_t)j * N, v[i], inv);
+    }
+    for (uint32_t j = threadIdx.x + kHold * kQuantThreads; j < nv; j += kQuantThreads) {
+        Vec<T> u;
+        u.raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
+        put_quant(qr + (uint64_t)j * N, u, inv);
+    }
+    for (uint32_t c = nv * N + threadIdx.x; c < k; c += kQuantThreads) qr[c] = (int8_t)quant_one(to_f32(xr[c]), inv);
+    if (threadIdx.x == 0) scale[blockIdx.x] = s;
 }
 
 struct Args {
@@ -93,6 +154,251 @@ __global__ void __launch_bounds__(256) k_w8a8_dp4a(Args a) {
             if (r < a.m && c < a.n)
                 put((T*)a.out + r * a.ld_o + c, __fmul_rn((float)acc[i][j], __fmul_rn(a.ws[c], a.as[r])));
         }
+}
+
+// ---- tensor cores: 128 tokens x BN channels per tile ----
+//
+// Persistent, one CTA per SM: warp 0 brings stages of 128 bytes of K (TMA, 128-byte swizzle; what lies
+// past a matrix's edge arrives as zeros, which add nothing), warp 1 owns TMEM and issues
+// tcgen05.mma kind::i8 (M = 128 tokens, N = BN channels, int32 sums), warps 2-5 read the sums of the
+// previous tile back (tcgen05.ld, thread = token), scale and store them, so two accumulator sets are
+// in flight.  Every wait is bounded; on a timeout the CTA sets bit 1 of the error word, drains its
+// copies and frees its TMEM.
+constexpr int kTileM = 128, kTileK = 128;
+constexpr int kTcThreads = 192;
+constexpr long long kWaitCycles = 4000000000ll;   // about 2 s
+
+template <int BN>
+__host__ __device__ constexpr int stages() { return BN == 256 ? 4 : BN == 128 ? 6 : 8; }
+
+template <int BN>
+struct alignas(1024) TcSmem {
+    int8_t a[stages<BN>()][kTileM * kTileK];
+    int8_t b[stages<BN>()][BN * kTileK];
+    uint8_t out[4][2][32 * 128];   // each epilogue warp: two boxes of 32 rows x 128 bytes, swizzled
+    float ws[BN];
+    uint64_t full[stages<BN>()], empty[stages<BN>()];
+    uint64_t tfull[2], tempty[2];
+    uint32_t tmem;
+    int abort;
+};
+template <int BN>
+__host__ __device__ constexpr size_t tc_smem() { return sizeof(TcSmem<BN>) + 1024; }
+
+struct TcArgs {
+    const float *as, *ws;
+    void* out;
+    uint64_t ld_o;
+    uint32_t m, n, k, tiles_m, tiles_n;
+    int tma_out;        // the output can be stored by TMA (16-byte aligned rows)
+    uint32_t* err;
+};
+
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (uint32_t i = 1;; i++) {
+        if (tc::mbar_try_wait(bar, parity)) return true;
+        if ((i & 255) == 0) {
+            if (*abort) return false;
+            if (clock64() - t0 > kWaitCycles) {
+                *abort = 1;
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ void drain_bar(uint64_t* bar, uint32_t parity) {   // ignores the abort flag
+    const long long t0 = clock64();
+    while (!tc::mbar_try_wait(bar, parity) && clock64() - t0 < kWaitCycles) {
+    }
+}
+
+// K-major operand in the 128-byte swizzle: rows of 128 bytes, 8-row atoms of 1,024 bytes.
+__device__ __forceinline__ uint64_t sw128_desc(const void* p) {
+    uint64_t d = (tc::smem_u32(p) >> 4) & 0x3FFFull;
+    d |= (uint64_t)1 << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+// Tiles in bands of 16 row tiles, column by column inside a band: the tiles in flight share both
+// operands in L2.
+__device__ __forceinline__ void tile_at(uint32_t t, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
+    const uint32_t band = t / (16 * tiles_n), in = t - band * 16 * tiles_n;
+    const uint32_t h = min(16u, tiles_m - band * 16);
+    tn = in / h;
+    tm = band * 16 + (in - tn * h);
+}
+
+template <int BN, class T>
+__global__ void __launch_bounds__(kTcThreads, 1)
+k_w8a8_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+          const __grid_constant__ CUtensorMap map_o, TcArgs g) {
+    extern __shared__ uint8_t raw[];
+    using S = TcSmem<BN>;
+    S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    constexpr int ST = stages<BN>();
+    constexpr uint32_t kStage = (kTileM + BN) * kTileK;
+    constexpr uint32_t kCols = 2 * BN < 32 ? 32 : 2 * BN;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t kb = (g.k + kTileK - 1) / kTileK, tiles = g.tiles_m * g.tiles_n;
+    volatile int* abort = &sm.abort;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; i++) {
+            tc::mbar_init(&sm.full[i], 1);
+            tc::mbar_init(&sm.empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            tc::mbar_init(&sm.tfull[i], 1);
+            tc::mbar_init(&sm.tempty[i], 4);
+        }
+        sm.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&sm.tmem)), "r"(kCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    tc::grid_wait();   // the activations may come from the preceding kernel
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                uint32_t tm, tn;
+                tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
+                for (uint32_t j = 0; j < kb; j++, it++) {
+                    const uint32_t s = it % ST;
+                    if (!wait_bar(&sm.empty[s], ((it / ST) & 1) ^ 1, abort)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::mbar_expect_tx(&sm.full[s], kStage);
+                    tc::tma_load_2d(sm.a[s], &map_a, (int)(j * kTileK), (int)(tm * kTileM), &sm.full[s]);
+                    tc::tma_load_2d(sm.b[s], &map_w, (int)(j * kTileK), (int)(tn * BN), &sm.full[s]);
+                }
+            }
+            if (!ok)   // the copies in flight land before the shared memory goes away
+                for (uint32_t i = it > ST ? it - ST : 0; i < it; i++) drain_bar(&sm.full[i % ST], (i / ST) & 1);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+            uint32_t it = 0, n = 0;
+            bool ok = true;
+            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, n++) {
+                const uint32_t buf = n & 1;
+                if (!wait_bar(&sm.tempty[buf], ((n >> 1) & 1) ^ 1, abort)) break;
+                tc::tc_fence_after();
+                const uint32_t d = tmem + buf * BN;
+                for (uint32_t j = 0; j < kb; j++, it++) {
+                    const uint32_t s = it % ST;
+                    if (!wait_bar(&sm.full[s], (it / ST) & 1, abort)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::tc_fence_after();
+                    const uint64_t da = sw128_desc(sm.a[s]), db = sw128_desc(sm.b[s]);
+#pragma unroll
+                    for (int ks = 0; ks < kTileK / 32; ks++) tc::mma_i8(d, da + 2 * ks, db + 2 * ks, idesc, (j | ks) != 0);
+                    tc::mma_commit(&sm.empty[s]);
+                }
+                if (ok) tc::mma_commit(&sm.tfull[buf]);
+            }
+            if (!ok || *abort) {   // no MMA may be running when TMEM is freed
+                for (uint32_t i = it > ST ? it - ST : 0; i < it; i++) drain_bar(&sm.empty[i % ST], (i / ST) & 1);
+            }
+        }
+        __syncwarp();
+    } else {
+        const int e = warp - 2, quad = warp & 3;
+        constexpr int kBox = 128 / (int)sizeof(T);   // columns of one 128-byte box row
+        uint32_t n = 0;
+        int ob = 0;
+        for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, n++) {
+            uint32_t tm, tn;
+            tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
+            const uint32_t buf = n & 1, n0 = tn * BN, row0 = tm * kTileM + quad * 32, row = row0 + lane;
+            asm volatile("bar.sync 1, 128;" ::: "memory");   // every epilogue warp is done with ws
+            for (int c = threadIdx.x - 64; c < BN; c += 128) sm.ws[c] = n0 + c < g.n ? g.ws[n0 + c] : 0.f;
+            const float as = row < g.m ? g.as[row] : 0.f;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (!wait_bar(&sm.tfull[buf], (n >> 1) & 1, abort)) break;
+            tc::tc_fence_after();
+            const uint32_t src = tmem + buf * BN + ((uint32_t)(quad * 32) << 16);
+            for (int c0 = 0; c0 < BN; c0 += kBox) {
+                if (n0 + c0 >= g.n) break;
+                uint8_t* box = sm.out[e][ob];
+                // TMA clips a store to 16 bytes: a box that the row's end cuts elsewhere is stored by lanes
+                const bool by_tma = g.tma_out && (n0 + c0 + kBox <= g.n || g.n % (16 / sizeof(T)) == 0);
+                if (g.tma_out) {   // the box's previous store has been read
+                    if (lane == 0) tc::bulk_wait_read<1>();
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int h = 0; h < kBox; h += 32) {
+                    int acc[32];
+                    tc::tmem_ld32(src + c0 + h, acc);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 16 / (int)sizeof(T)) {
+                        float y[16 / sizeof(T)];
+#pragma unroll
+                        for (int j = 0; j < 16 / (int)sizeof(T); j++)
+                            y[j] = __fmul_rn((float)acc[i + j], __fmul_rn(sm.ws[c0 + h + i + j], as));
+                        uint4 w;
+                        if constexpr (sizeof(T) == 4) {
+                            w = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+                        } else {
+                            __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) p[j] = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
+                        }
+                        const int chunk = (h + i) * (int)sizeof(T) / 16;
+                        *reinterpret_cast<uint4*>(box + lane * 128 + ((chunk ^ (lane & 7)) * 16)) = w;
+                    }
+                }
+                if (by_tma) {
+                    tc::fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (row0 < g.m) tc::tma_store_2d(&map_o, (int)(n0 + c0), (int)row0, box);
+                        tc::bulk_commit();
+                    }
+                    ob ^= 1;
+                } else {   // any stride and alignment: a row's columns by consecutive lanes
+                    __syncwarp();
+                    for (int r = 0; r < 32 && row0 + r < g.m; r++)
+                        for (int c = lane; c < kBox && n0 + c0 + c < g.n; c += 32) {
+                            const int chunk = c * (int)sizeof(T) / 16, in = c % (16 / (int)sizeof(T));
+                            ((T*)g.out)[(row0 + r) * g.ld_o + n0 + c0 + c] =
+                                reinterpret_cast<const T*>(box + r * 128 + ((chunk ^ (r & 7)) * 16))[in];
+                        }
+                    __syncwarp();
+                }
+            }
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&sm.tempty[buf]);
+        }
+        if (lane == 0) tc::bulk_wait<0>();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && sm.abort) atomicOr(g.err, 2u);
+    if (warp == 1) {
+        tc::tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+    }
 }
 
 }  // namespace w8
