@@ -11,6 +11,7 @@
 
 #include "../../include/redukt_gpu.h"
 #include "rk_delta.cuh"
+#include "rk_delta_chunk.cuh"
 #include "rk_error.h"
 #include "rk_plan.cuh"
 #include "rk_w8a8.cuh"
@@ -54,6 +55,12 @@ cudaError_t set_smem() {
     return cudaFuncSetAttribute(rk::w8::k_w8a8_tc<BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rk::w8::tc_smem<BN>());
 }
 
+template <int DK, class T>
+cudaError_t set_chunk_smem() {
+    return cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)sizeof(rk::delta::ChunkSmem<DK, T>));
+}
+
 // The current device's facts; the first call on a device looks them up and sets the kernels'
 // shared-memory limits.
 int32_t device(Device** out) {
@@ -68,6 +75,10 @@ int32_t device(Device** out) {
         d.err = static_cast<uint32_t*>(p);
         OP_CK(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
         OP_CK(cudaFuncSetAttribute(rk::plan::k_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::plan::Smem)));
+        OP_CK((set_chunk_smem<64, float>()));
+        OP_CK((set_chunk_smem<128, float>()));
+        OP_CK((set_chunk_smem<64, __nv_bfloat16>()));
+        OP_CK((set_chunk_smem<128, __nv_bfloat16>()));
         OP_CK((set_smem<256, float>()));
         OP_CK((set_smem<256, __nv_bfloat16>()));
         OP_CK((set_smem<128, float>()));
@@ -120,6 +131,15 @@ int32_t delta_args(const char* what, rk::delta::Args& a, const void* d_q, const 
     OP_REQUIRE(std::isfinite(scale), "%s: the scale is not finite", what);
     a = {d_q, d_k, d_v, d_log_decay, d_beta, nullptr, d_slots, d_fresh, n, n_rows, n_qk_heads, n_v_heads, d_value,
          ld_q, ld_k, ld_v, ld_gate, ld_out, scale, l2norm, d_state, n_slots, slot_stride, d_out, nullptr};
+    return BACKEND_OK;
+}
+
+template <int DK, class T>
+int32_t launch_chunk(const rk::delta::ChunkArgs& ca, cudaStream_t st) {
+    using namespace rk::delta;
+    const dim3 grid((unsigned)ceil_div(ca.a.dv, kVRows), ca.a.hv, ca.a.n);
+    k_delta_chunk<DK, T, 0><<<grid, kCThreads, sizeof(ChunkSmem<DK, T>), st>>>(ca);
+    OP_CK(cudaGetLastError());
     return BACKEND_OK;
 }
 
@@ -308,18 +328,10 @@ int32_t redukt_b200_delta_chunk(const void* d_q, const void* d_k, const void* d_
     if (int32_t rc = device(&d)) return rc;
     a.err = d->err;
     a.cu = d_cu;
-    const dim3 grid((d_value + rk::delta::kRows - 1) / rk::delta::kRows, n_v_heads, n_requests);
     const cudaStream_t st = stream_of(cuda_stream);
-    const int threads = rk::delta::kWarps * 32;
-    if (dtype == REDUKT_DTYPE_F32) {
-        if (d_key == 64) rk::delta::k_delta_serial<64, float><<<grid, threads, 0, st>>>(a);
-        else rk::delta::k_delta_serial<128, float><<<grid, threads, 0, st>>>(a);
-    } else {
-        if (d_key == 64) rk::delta::k_delta_serial<64, __nv_bfloat16><<<grid, threads, 0, st>>>(a);
-        else rk::delta::k_delta_serial<128, __nv_bfloat16><<<grid, threads, 0, st>>>(a);
-    }
-    OP_CK(cudaGetLastError());
-    return BACKEND_OK;
+    rk::delta::ChunkArgs ca = {a, nullptr, 0, 1, nullptr, nullptr, nullptr};
+    if (dtype == REDUKT_DTYPE_F32) return d_key == 64 ? launch_chunk<64, float>(ca, st) : launch_chunk<128, float>(ca, st);
+    return d_key == 64 ? launch_chunk<64, __nv_bfloat16>(ca, st) : launch_chunk<128, __nv_bfloat16>(ca, st);
 }
 
 int32_t redukt_b200_quantize_tokens(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q,
