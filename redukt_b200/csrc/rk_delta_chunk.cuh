@@ -40,6 +40,8 @@ __device__ __forceinline__ int strip_at(int row, int col) {
     return 16 * (8 * r + 8 * r * (r + 1)) + (row & 15) * (16 * r + 24) + col;
 }
 
+constexpr int kDiagLd = 20;         // rows of 16 floats on 16 bytes, two columns apart in other banks
+
 template <int DK, class T>
 struct ChunkCfg {
     static constexpr bool kF32 = sizeof(T) == 4;
@@ -55,12 +57,14 @@ struct alignas(16) ChunkSmem {
     __half q[Cfg::KP][kC * Cfg::LD];
     __half m[2][kStripHalves];          // A below the diagonal blocks, their inverses on them
     __half p[2][kStripHalves];
-    float diag[kCWarps][16 * 17];       // a diagonal block, transposed: [column][row]
+    float diag[kCWarps][16 * kDiagLd];  // a diagonal block, transposed: [column][row]
     float sk[kC], sq[kC];               // row scales of the planes, norms folded in
     float chi[kC], clo[kC];             // c * log2(e) in two floats
     float beta[kC];
     float ak[kC], cq[kC], wk[kC];       // factors of X, O and the update, per token
-    float arow[kC], prow[kC];           // row scales of A and P
+    float rf[kC];                       // e^{c_i - c_ref}, ref = the token before i's strip
+    float cf[3][kC];                    // strip r + 1: e^{c_ref - c_j} times the key's scale
+    float ascale[4][kC], pscale[4][kC]; // scales of a row of each 16 x 16 block of A and P
     float dblk[kCWarps];                // scale of each inverted block
     float gamma;
 };
@@ -112,6 +116,8 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const __half* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(tc::smem_u32(p)) : "memory");
 }
+
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // One row of DK values of type T to f16 planes: 8 lanes a row, lane l of the eight takes the 16-byte
 // vectors l, l + 8, ...  Returns the row's scale (its inverse power of two, times 1 / norm).
@@ -227,99 +233,140 @@ __device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& 
     }
     __syncthreads();
     if (threadIdx.x < kC) {
-        const int i = threadIdx.x;
+        const int i = threadIdx.x, ref = (i & ~15) - 1;
         const float c = sm.chi[i] + sm.clo[i], e = exp2f(c);
         const float w = exp2f((sm.chi[kC - 1] - sm.chi[i]) + (sm.clo[kC - 1] - sm.clo[i]));
         sm.ak[i] = e * sm.sk[i];
         sm.wk[i] = w * sm.sk[i];
         if (kOut) sm.cq[i] = a.scale * e * sm.sq[i];
         if (i == kC - 1) sm.gamma = e;
+        sm.rf[i] = ref < 0 ? 1.f : exp2f((sm.chi[i] - sm.chi[max(ref, 0)]) + (sm.clo[i] - sm.clo[max(ref, 0)]));
+    } else {
+        const int j = threadIdx.x - kC;
+#pragma unroll
+        for (int r = 1; r < 4; r++)
+            if (j < 16 * r) sm.cf[r - 1][j] = sm.sk[j] * exp2f((sm.chi[16 * r - 1] - sm.chi[j]) + (sm.clo[16 * r - 1] - sm.clo[j]));
     }
-    // Rows 16 r .. 16 r + 15 against tokens 0 .. 16 r + 15: warp w does strip w of K K^T and strip
-    // 3 - w of Q K^T, which is the same work for every warp.
-#pragma unroll 1
-    for (int what = 0; what < (kOut ? 2 : 1); what++) {
-        const int r = what ? kCWarps - 1 - warp : warp;
-        const __half* ap = what ? sm.q[0] : sm.k[0];
-        const __half* al = what ? sm.q[KP - 1] : sm.k[KP - 1];
-        float acc[8][4];
+    // Strip r of a product is rows 16 r .. 16 r + 15 against tokens 0 .. 16 r + 15.  Warp w does strip w of
+    // K K^T and strip 3 - w of Q K^T, five 16 x 16 blocks for every warp: slot 0 the diagonal block of the
+    // first, slot 1 that of the second, slots 2-4 the blocks beside them.
+    const int rg = warp, rh = kCWarps - 1 - warp;
+    float acc[5][2][4];
 #pragma unroll
-        for (int n = 0; n < 8; n++)
+    for (int s = 0; s < 5; s++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) acc[n][c] = 0.f;
-        const int arow = 16 * r + (lane & 7) + ((lane >> 3) & 1) * 8, acol = (lane >> 4) * 8;
+        for (int c = 0; c < 4; c++) acc[s][0][c] = acc[s][1][c] = 0.f;
+    {
+        const int arow = (lane & 7) + ((lane >> 3) & 1) * 8, acol = (lane >> 4) * 8;
         const int brow = (lane & 7) + (lane >> 4) * 8, bcol = ((lane >> 3) & 1) * 8;
 #pragma unroll
         for (int ks = 0; ks < DK / 16; ks++) {
-            uint32_t fa[4], fl[4];
-            ldsm4(fa, ap + arow * LD + ks * 16 + acol);
-            if (KP == 2) ldsm4(fl, al + arow * LD + ks * 16 + acol);
+            uint32_t fk[4], fkl[4], fq[4], fql[4];
+            ldsm4(fk, &sm.k[0][(16 * rg + arow) * LD + ks * 16 + acol]);
+            if (KP == 2) ldsm4(fkl, &sm.k[KP - 1][(16 * rg + arow) * LD + ks * 16 + acol]);
+            if (kOut) {
+                ldsm4(fq, &sm.q[0][(16 * rh + arow) * LD + ks * 16 + acol]);
+                if (KP == 2) ldsm4(fql, &sm.q[KP - 1][(16 * rh + arow) * LD + ks * 16 + acol]);
+            }
 #pragma unroll
-            for (int nn = 0; nn < 4; nn++) {
-                if (nn > r) continue;
-                uint32_t fb[4];
-                ldsm4(fb, &sm.k[0][(nn * 16 + brow) * LD + ks * 16 + bcol]);
+            for (int s = 0; s < 5; s++) {
+                const bool key = s == 0 || (s > 1 && s - 2 < warp);
+                if (!kOut && !key) continue;
+                const int nb = s == 0 ? rg : s == 1 ? rh : s - 2 < warp ? s - 2 : s - 2 - warp;
+                uint32_t fa[4], fl[4], fb[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    fa[c] = !kOut || key ? fk[c] : fq[c];
+                    if (KP == 2) fl[c] = !kOut || key ? fkl[c] : fql[c];
+                }
+                const int off = (nb * 16 + brow) * LD + ks * 16 + bcol;
+                ldsm4(fb, &sm.k[0][off]);
                 if (KP == 2) {
                     uint32_t fw[4];
-                    ldsm4(fw, &sm.k[KP - 1][(nn * 16 + brow) * LD + ks * 16 + bcol]);
-                    mma_f16(acc[2 * nn], fa, fw[0], fw[1]);
-                    mma_f16(acc[2 * nn + 1], fa, fw[2], fw[3]);
-                    mma_f16(acc[2 * nn], fl, fb[0], fb[1]);
-                    mma_f16(acc[2 * nn + 1], fl, fb[2], fb[3]);
+                    ldsm4(fw, &sm.k[KP - 1][off]);
+                    mma_f16(acc[s][0], fa, fw[0], fw[1]);
+                    mma_f16(acc[s][1], fa, fw[2], fw[3]);
+                    mma_f16(acc[s][0], fl, fb[0], fb[1]);
+                    mma_f16(acc[s][1], fl, fb[2], fb[3]);
                 }
-                mma_f16(acc[2 * nn], fa, fb[0], fb[1]);
-                mma_f16(acc[2 * nn + 1], fa, fb[2], fb[3]);
+                mma_f16(acc[s][0], fa, fb[0], fb[1]);
+                mma_f16(acc[s][1], fa, fb[2], fb[3]);
             }
         }
-        // this thread: rows i0 = 16 r + g and i1 = i0 + 8, columns 8 n + 2 t, + 1
-        const int i0 = 16 * r + g, i1 = i0 + 8;
-        const float s0 = what ? a.scale * sm.sq[i0] : sm.beta[i0] * sm.sk[i0];
-        const float s1 = what ? a.scale * sm.sq[i1] : sm.beta[i1] * sm.sk[i1];
-        float m0 = 0.f, m1 = 0.f;
+    }
+    __syncthreads();   // the factors below
+    {
+        const int ig = 16 * rg + g, ih = 16 * rh + g;
+        const float kg0 = sm.beta[ig] * sm.sk[ig], kg1 = sm.beta[ig + 8] * sm.sk[ig + 8];
+        const float kh0 = kOut ? a.scale * sm.sq[ih] : 0.f, kh1 = kOut ? a.scale * sm.sq[ih + 8] : 0.f;
+        // diagonal blocks: every pair's own exponent (column 8 n + 2 t + c of the block, rows g and g + 8)
 #pragma unroll
-        for (int n = 0; n < 8; n++) {
-            if (n > 2 * r + 1) continue;
-            const int j = 8 * n + 2 * t;
+        for (int s = 0; s < (kOut ? 2 : 1); s++) {
+            const int i0 = s ? ih : ig, base = 16 * (s ? rh : rg);
+            const float r0 = s ? kh0 : kg0, r1 = s ? kh1 : kg1;
+            const float ch0 = sm.chi[i0], cl0 = sm.clo[i0], ch1 = sm.chi[i0 + 8], cl1 = sm.clo[i0 + 8];
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const float kj = sm.sk[j + c], h0 = sm.chi[j + c], l0 = sm.clo[j + c];
-                const bool in0 = what ? j + c <= i0 : j + c < i0, in1 = what ? j + c <= i1 : j + c < i1;
-                acc[n][c] = in0 ? acc[n][c] * (s0 * kj) * exp2f((sm.chi[i0] - h0) + (sm.clo[i0] - l0)) : 0.f;
-                acc[n][2 + c] = in1 ? acc[n][2 + c] * (s1 * kj) * exp2f((sm.chi[i1] - h0) + (sm.clo[i1] - l0)) : 0.f;
-                if (what || n < 2 * r) {
-                    m0 = amax(m0, acc[n][c]);
-                    m1 = amax(m1, acc[n][2 + c]);
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int jj = 8 * n + 2 * t + c, j = base + jj;
+                    const float kj = sm.sk[j], h = sm.chi[j], w = sm.clo[j];
+                    const float e0 = exp2f((ch0 - h) + (cl0 - w)), e1 = exp2f((ch1 - h) + (cl1 - w));
+                    const bool in0 = s ? jj <= g : jj < g, in1 = s ? jj <= g + 8 : jj < g + 8;
+                    acc[s][n][c] = in0 ? acc[s][n][c] * (r0 * kj) * e0 : 0.f;
+                    acc[s][n][2 + c] = in1 ? acc[s][n][2 + c] * (r1 * kj) * e1 : 0.f;
+                    if (s == 0) {
+                        sm.diag[warp][jj * kDiagLd + g] = acc[0][n][c];
+                        sm.diag[warp][jj * kDiagLd + g + 8] = acc[0][n][2 + c];
+                    }
                 }
-            }
         }
-        float v0, v1;
-        const float p0 = row_pow(quad_max(m0), v0), p1 = row_pow(quad_max(m1), v1);
-        if (t == 0) {
-            (what ? sm.prow : sm.arow)[i0] = v0;
-            (what ? sm.prow : sm.arow)[i1] = v1;
-        }
-        __half* hi = what ? sm.p[0] : sm.m[0];
-        __half* lo = what ? sm.p[1] : sm.m[1];
+        // the blocks beside them: a factor per row and one per column
+        const float fg0 = kg0 * sm.rf[ig], fg1 = kg1 * sm.rf[ig + 8], fh0 = kh0 * sm.rf[ih], fh1 = kh1 * sm.rf[ih + 8];
 #pragma unroll
-        for (int n = 0; n < 8; n++) {
-            if (n > 2 * r + 1) continue;
-            const int j = 8 * n + 2 * t;
-            if (!what && n >= 2 * r) {   // the diagonal block is inverted below
-                const int jj = j - 16 * r;
-                sm.diag[warp][jj * 17 + g] = acc[n][0];
-                sm.diag[warp][(jj + 1) * 17 + g] = acc[n][1];
-                sm.diag[warp][jj * 17 + g + 8] = acc[n][2];
-                sm.diag[warp][(jj + 1) * 17 + g + 8] = acc[n][3];
-                continue;
+        for (int s = 1; s < 5; s++) {
+            const bool key = s > 1 && s - 2 < warp;
+            if (!kOut && !key) continue;
+            const int nb = s == 1 ? rh : key ? s - 2 : s - 2 - warp;
+            const int r = key ? rg : rh, i0 = 16 * r + g;
+            if (s > 1) {
+                const float* cf = sm.cf[r - 1] + 16 * nb + 2 * t;
+                const float r0 = key ? fg0 : fh0, r1 = key ? fg1 : fh1;
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        acc[s][n][c] *= r0 * cf[8 * n + c];
+                        acc[s][n][2 + c] *= r1 * cf[8 * n + c];
+                    }
             }
-            uint32_t x, y;
-            const int at0 = strip_at(i0, j), at1 = strip_at(i1, j);
-            split2(acc[n][0] * p0, acc[n][1] * p0, x, y);
-            *reinterpret_cast<uint32_t*>(hi + at0) = x;
-            *reinterpret_cast<uint32_t*>(lo + at0) = y;
-            split2(acc[n][2] * p1, acc[n][3] * p1, x, y);
-            *reinterpret_cast<uint32_t*>(hi + at1) = x;
-            *reinterpret_cast<uint32_t*>(lo + at1) = y;
+            float m0 = 0.f, m1 = 0.f, v0, v1;
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    m0 = amax(m0, acc[s][n][c]);
+                    m1 = amax(m1, acc[s][n][2 + c]);
+                }
+            const float p0 = row_pow(quad_max(m0), v0), p1 = row_pow(quad_max(m1), v1);
+            float* sc = key ? sm.ascale[nb] : sm.pscale[nb];
+            if (t == 0) {
+                sc[i0] = v0;
+                sc[i0 + 8] = v1;
+            }
+            __half* hi = key ? sm.m[0] : sm.p[0];
+            __half* lo = key ? sm.m[1] : sm.p[1];
+            const int at = strip_at(i0, 16 * nb + 2 * t), down = 8 * (16 * r + 24);
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                uint32_t x, y;
+                split2(acc[s][n][0] * p0, acc[s][n][1] * p0, x, y);
+                *reinterpret_cast<uint32_t*>(hi + at + 8 * n) = x;
+                *reinterpret_cast<uint32_t*>(lo + at + 8 * n) = y;
+                split2(acc[s][n][2] * p1, acc[s][n][3] * p1, x, y);
+                *reinterpret_cast<uint32_t*>(hi + at + down + 8 * n) = x;
+                *reinterpret_cast<uint32_t*>(lo + at + down + 8 * n) = y;
+            }
         }
     }
     __syncwarp();
@@ -330,9 +377,16 @@ __device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& 
 #pragma unroll
         for (int i = 0; i < 16; i++) x[i] = i == c ? 1.f : 0.f;
 #pragma unroll
-        for (int j = 0; j < 15; j++)
+        for (int j = 0; j < 15; j++) {
+            float col[16];
 #pragma unroll
-            for (int i = j + 1; i < 16; i++) x[i] = fmaf(-at[j * 17 + i], x[j], x[i]);
+            for (int i = (j + 1) & ~3; i < 16; i += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(at + j * kDiagLd + i);
+                col[i] = f.x, col[i + 1] = f.y, col[i + 2] = f.z, col[i + 3] = f.w;
+            }
+#pragma unroll
+            for (int i = j + 1; i < 16; i++) x[i] = fmaf(-col[i], x[j], x[i]);
+        }
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; i++) m = amax(m, x[i]);
@@ -458,6 +512,21 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
     for (uint64_t at = t0; at < t1; at += kC) {
         const int len = (int)min((uint64_t)kC, t1 - at);
         prepare_chunk<DK, T, kOut>(sm, a, at, len, h, hq, wide);
+        if (at + kC < t1) {   // the next chunk's rows on their way to L2
+            const uint64_t r = at + kC + (threadIdx.x >> 1);
+            if (r < t1) {
+                const char* kn = (const char*)((const T*)a.k + r * a.ld_k + (uint64_t)hq * DK);
+                const char* qn = (const char*)((const T*)a.q + r * a.ld_q + (uint64_t)hq * DK);
+#pragma unroll
+                for (int b = 0; b < DK * (int)sizeof(T); b += 256) {
+                    const int o = b + (threadIdx.x & 1) * 128;
+                    if (o < DK * (int)sizeof(T)) {
+                        prefetch_l2(kn + o);
+                        if (kOut) prefetch_l2(qn + o);
+                    }
+                }
+            }
+        }
         if (active) {
             // X = S K^T and O = S Q^T over the 64 tokens; V meanwhile
             T V[8][4];
@@ -541,8 +610,8 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
                     mma_block(d0, d1, uh[jb], ul[jb], sm.m[0], sm.m[1], ib, jb, lane);
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
-                        r0[c] = fmaf(-(sm.arow[i + (c & 1)] * us[jb][c >> 1]), d0[c], r0[c]);
-                        r1[c] = fmaf(-(sm.arow[i + 8 + (c & 1)] * us[jb][c >> 1]), d1[c], r1[c]);
+                        r0[c] = fmaf(-(sm.ascale[jb][i + (c & 1)] * us[jb][c >> 1]), d0[c], r0[c]);
+                        r1[c] = fmaf(-(sm.ascale[jb][i + 8 + (c & 1)] * us[jb][c >> 1]), d1[c], r1[c]);
                     }
                 }
                 uint32_t hi[4], lo[4];
@@ -564,8 +633,8 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
                         mma_block(e0, e1, uh[jb], ul[jb], sm.p[0], sm.p[1], ib, jb, lane);
 #pragma unroll
                         for (int c = 0; c < 4; c++) {
-                            O[2 * ib][c] = fmaf(sm.prow[i + (c & 1)] * us[jb][c >> 1], e0[c], O[2 * ib][c]);
-                            O[2 * ib + 1][c] = fmaf(sm.prow[i + 8 + (c & 1)] * us[jb][c >> 1], e1[c], O[2 * ib + 1][c]);
+                            O[2 * ib][c] = fmaf(sm.pscale[jb][i + (c & 1)] * us[jb][c >> 1], e0[c], O[2 * ib][c]);
+                            O[2 * ib + 1][c] = fmaf(sm.pscale[jb][i + 8 + (c & 1)] * us[jb][c >> 1], e1[c], O[2 * ib + 1][c]);
                         }
                     }
                 }
