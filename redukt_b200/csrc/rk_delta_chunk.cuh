@@ -120,47 +120,49 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const __half* p) {
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // One row of DK values of type T to f16 planes: 8 lanes a row, lane l of the eight takes the 16-byte
-// vectors l, l + 8, ...  Returns the row's scale (its inverse power of two, times 1 / norm).
+// vectors l, l + 8, ...
 template <int DK, class T>
 struct RowLoad {
     static constexpr int N = 16 / sizeof(T), NV = DK / N / 8;
     uint4 raw[NV];
-    __device__ __forceinline__ void load(const T* p, bool live, bool wide, int l) {
+    __device__ __forceinline__ void load(const T* p, int l) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) raw[i] = *reinterpret_cast<const uint4*>(p + (l + 8 * i) * N);
+    }
+    __device__ __forceinline__ void load_single(const T* p, int l) {   // any alignment
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < N; c++) reinterpret_cast<T*>(&raw[i])[c] = p[(l + 8 * i) * N + c];
+    }
+    __device__ __forceinline__ void clear_unless(bool live) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            raw[i] = make_uint4(0, 0, 0, 0);
-            const T* s = p + (l + 8 * i) * N;
-            if (live && wide) raw[i] = *reinterpret_cast<const uint4*>(s);
-            else if (live)
-#pragma unroll
-                for (int c = 0; c < N; c++) reinterpret_cast<T*>(&raw[i])[c] = s[c];
+            raw[i].x = live ? raw[i].x : 0u;
+            raw[i].y = live ? raw[i].y : 0u;
+            raw[i].z = live ? raw[i].z : 0u;
+            raw[i].w = live ? raw[i].w : 0u;
         }
     }
-    __device__ __forceinline__ float put(__half* hi, __half* lo, bool l2norm, int l) const {
-        float m = 0.f, ss = 0.f;
+    __device__ __forceinline__ float get(int i, int c) const { return to_f32(reinterpret_cast<const T*>(&raw[i])[c]); }
+    __device__ __forceinline__ void sums(float& m, float& ss) const {   // this lane's part
+        m = ss = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
             for (int c = 0; c < N; c++) {
-                const float x = to_f32(reinterpret_cast<const T*>(&raw[i])[c]);
-                m = amax(m, x);
-                ss = fmaf(x, x, ss);
+                m = amax(m, get(i, c));
+                ss = fmaf(get(i, c), get(i, c), ss);
             }
-        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
-        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-        float inv;
-        const float s = row_pow(m, inv);
-        if (l2norm) inv *= 1.f / sqrtf(sum8(ss) + kNormEps);
+    }
+    __device__ __forceinline__ void put(__half* hi, __half* lo, float s, int l) const {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             uint32_t h[N / 2], w[N / 2];
 #pragma unroll
             for (int c = 0; c < N / 2; c++) {
-                const float x = s * to_f32(reinterpret_cast<const T*>(&raw[i])[2 * c]);
-                const float y = s * to_f32(reinterpret_cast<const T*>(&raw[i])[2 * c + 1]);
-                if constexpr (sizeof(T) == 4) split2(x, y, h[c], w[c]);
-                else h[c] = pack_hi(x, y);
+                if constexpr (sizeof(T) == 4) split2(s * get(i, 2 * c), s * get(i, 2 * c + 1), h[c], w[c]);
+                else h[c] = pack_hi(s * get(i, 2 * c), s * get(i, 2 * c + 1));
             }
             const int at = (l + 8 * i) * N;
             if constexpr (sizeof(T) == 4) {
@@ -170,9 +172,36 @@ struct RowLoad {
                 *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
             }
         }
-        return inv;
     }
 };
+
+// Four rows of each 8-lane group: r, r + 4, r + 8, r + 12 of the warp's 16.
+template <int DK, class T>
+__device__ __forceinline__ void put_rows(RowLoad<DK, T> (&x)[4], __half* hi, __half* lo, int ld, float* scale, int row, int len, bool l2norm, int l) {
+    float m[4], ss[4], s[4], inv[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[i].clear_unless(row + 4 * i < len);
+        x[i].sums(m[i], ss[i]);
+    }
+#pragma unroll
+    for (int o = 4; o; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; i++) m[i] = fmaxf(m[i], __shfl_xor_sync(0xFFFFFFFFu, m[i], o));
+    if (l2norm) {
+#pragma unroll
+        for (int o = 4; o; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < 4; i++) ss[i] += __shfl_xor_sync(0xFFFFFFFFu, ss[i], o);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        s[i] = row_pow(m[i], inv[i]);
+        if (l2norm) inv[i] *= 1.f / sqrtf(ss[i] + kNormEps);
+        x[i].put(hi + (row + 4 * i) * ld, lo + (row + 4 * i) * ld, s[i], l);
+        if (l == 0) scale[row + 4 * i] = inv[i];
+    }
+}
 
 // Fills the chunk's shared operands: planes and scales of k and q, decay factors, A, its inverted
 // diagonal blocks, and P.  All warps; ends with a barrier.
@@ -183,14 +212,20 @@ __device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& 
     constexpr int LD = Cfg::LD, KP = Cfg::KP;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane >> 3, l = lane & 7, g = lane >> 2, t = lane & 3;
     {
-        const T* kp = (const T*)a.k + (uint64_t)hq * DK;
-        const T* qp = (const T*)a.q + (uint64_t)hq * DK;
+        const T* kp = (const T*)a.k + t0 * a.ld_k + (uint64_t)hq * DK;
+        const T* qp = (const T*)a.q + t0 * a.ld_q + (uint64_t)hq * DK;
+        const int row = warp * 16 + grp;
         RowLoad<DK, T> rk[4], rq[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = warp * 16 + 4 * i + grp;
-            rk[i].load(kp + (t0 + r) * a.ld_k, r < len, wide, l);
-            if (kOut) rq[i].load(qp + (t0 + r) * a.ld_q, r < len, wide, l);
+        for (int i = 0; i < 4; i++) {   // rows past the end read the last one and are cleared
+            const uint32_t r = min(row + 4 * i, len - 1);
+            if (wide) {
+                rk[i].load(kp + r * a.ld_k, l);
+                if (kOut) rq[i].load(qp + r * a.ld_q, l);
+            } else {
+                rk[i].load_single(kp + r * a.ld_k, l);
+                if (kOut) rq[i].load_single(qp + r * a.ld_q, l);
+            }
         }
         if (warp == 0) {   // tokens 2 lane, 2 lane + 1
             double c0 = 0.0, c1 = 0.0;
@@ -220,16 +255,8 @@ __device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& 
             sm.beta[i0] = b0;
             sm.beta[i0 + 1] = b1;
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = warp * 16 + 4 * i + grp;
-            const float s = rk[i].put(&sm.k[0][r * LD], &sm.k[KP - 1][r * LD], a.l2norm, l);
-            if (l == 0) sm.sk[r] = s;
-            if (kOut) {
-                const float z = rq[i].put(&sm.q[0][r * LD], &sm.q[KP - 1][r * LD], a.l2norm, l);
-                if (l == 0) sm.sq[r] = z;
-            }
-        }
+        put_rows<DK, T>(rk, sm.k[0], sm.k[KP - 1], LD, sm.sk, row, len, a.l2norm, l);
+        if (kOut) put_rows<DK, T>(rq, sm.q[0], sm.q[KP - 1], LD, sm.sq, row, len, a.l2norm, l);
     }
     __syncthreads();
     if (threadIdx.x < kC) {
