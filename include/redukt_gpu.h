@@ -305,8 +305,9 @@ int32_t redukt_b200_delta_step(const void* d_q, const void* d_k, const void* d_v
  * above it is touched.  A request without tokens keeps its state (fresh: zero state).  The same
  * call gives the same bits every time; they are near, not equal to, n calls of delta_step.
  * d_blocks (block, max_blocks) is the plan's block table, used to cut long requests where there are
- * few of them; NULL = never cut.  d_work: redukt_b200_delta_work_bytes() bytes on 256; with less
- * (NULL and 0 among it) requests are not cut. */
+ * few of them; NULL = never cut (block a multiple of 64, max_blocks at most 65,535 and at least
+ * n_tokens / block + n_requests).  d_work on 256 bytes: redukt_b200_delta_work_bytes() let requests be
+ * cut at every block, fewer bytes at fewer of them; NULL = never cut. */
 int32_t redukt_b200_delta_chunk(const void* d_q, const void* d_k, const void* d_v, int32_t dtype, const float* d_log_decay,
                                 const float* d_beta, uint32_t n_tokens, uint32_t n_requests, const uint32_t* d_cu,
                                 const uint32_t* d_slots, const uint32_t* d_fresh, uint32_t n_qk_heads, uint32_t n_v_heads,

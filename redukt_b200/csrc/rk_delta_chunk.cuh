@@ -71,10 +71,21 @@ struct alignas(16) ChunkSmem {
 
 struct ChunkArgs {
     Args a;
-    const uint32_t* blocks;       // (request, index) of each block; NULL = one block per request
+    const uint32_t* blocks;       // (request, index) of each table block
     uint32_t block, merge;        // tokens per table block; table blocks per segment
     float *b_seg, *m_seg, *s_in;  // per segment and head: end state from zero, transition, start state
 };
+
+// A cut request: segments of block * merge tokens.  Over a segment a state row s becomes s M + b with M
+// and b of that segment alone (M: what the rows of the identity become with v = 0; b: what zero
+// becomes), so three launches replace the chain: the segments' M and b side by side, the start
+// states one after the other (k_delta_scan, one small product per segment), the segments with
+// outputs side by side.
+// Number of a segment in the workspace: different for every (request, index / merge), and below
+// n_rows / (block * merge) + n, because a request of l tokens has at most l / seg + 1 segments.
+__device__ __forceinline__ uint64_t segment_id(const ChunkArgs& c, uint64_t first_row, uint32_t req, uint32_t seg_index) {
+    return first_row / ((uint64_t)c.block * c.merge) + req + seg_index;
+}
 
 // 2^(14 - e) for a largest magnitude in [2^e, 2^(e+1)), and its inverse; finite for every m.
 __device__ __forceinline__ float row_pow(float m, float& inv) {
@@ -490,6 +501,7 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
     }
     const uint32_t slot = a.slots[req];
     uint64_t t0 = min(a.cu[req], a.n_rows), t1 = min(a.cu[req + 1], a.n_rows);
+    const uint64_t seg_head = kMode == 0 ? 0 : segment_id(ca, t0, req, index / ca.merge) * a.hv + h;
     bool last = true;
     if (kMode != 0) {
         const uint64_t seg = (uint64_t)ca.block * ca.merge, b = t0 + (uint64_t)index * ca.block;
@@ -511,7 +523,7 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
     }
     const bool ident = kMode == 1 && row0 >= (int)a.dv;
     const bool active = row0 < (int)a.dv + (kMode == 1 ? DK : 0);
-    const uint64_t per_head = (uint64_t)a.dv * DK, seg_head = (uint64_t)blockIdx.z * a.hv + h;
+    const uint64_t per_head = (uint64_t)a.dv * DK;
     float* st = a.state + slot * a.slot_stride + h * per_head;
     const float* src = kMode == 2 ? ca.s_in + seg_head * per_head : st;
     const bool zero = kMode == 1 || (kMode == 0 && a.fresh && a.fresh[req]);
@@ -729,7 +741,7 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
         }
         __syncthreads();   // the shared operands are free again
     }
-    if (!active || (kMode == 2 && !last)) return;
+    if (!active || (kMode == 2 && !last)) return;   // only the last segment's end is the request's
     float* dst = st;
     int r = row0;
     if (kMode == 1) {
@@ -741,6 +753,51 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
         const int c = 8 * n + 2 * t;
         *reinterpret_cast<float2*>(dst + (uint64_t)(r + g) * DK + c) = make_float2(S[n][0], S[n][1]);
         *reinterpret_cast<float2*>(dst + (uint64_t)(r + g + 8) * DK + c) = make_float2(S[n][2], S[n][3]);
+    }
+}
+
+// Start states of a request's segments: S, S M_0 + b_0, ...  grid (ceil(dv / 8), hv, requests), DK threads:
+// thread j owns column j of 8 state rows; bound by the L2 reads of M (DK^2 floats per segment and block).
+constexpr int kScanRows = 8;
+template <int DK>
+__global__ void __launch_bounds__(DK) k_delta_scan(ChunkArgs ca) {
+    __shared__ float4 rows[kScanRows][DK / 4];
+    const Args& a = ca.a;
+    const uint32_t h = blockIdx.y, req = blockIdx.z, slot = a.slots[req], j = threadIdx.x, r0 = blockIdx.x * kScanRows;
+    const uint64_t t0 = min(a.cu[req], a.n_rows), t1 = min(a.cu[req + 1], a.n_rows), seg = (uint64_t)ca.block * ca.merge;
+    if (slot >= a.n_slots || t0 >= t1) {   // a fresh request without tokens still leaves a zero state
+        if (slot < a.n_slots && a.fresh && a.fresh[req])
+            for (int r = 0; r < kScanRows; r++) a.state[slot * a.slot_stride + ((uint64_t)h * a.dv + r0 + r) * DK + j] = 0.f;
+        return;
+    }
+    const uint64_t per_head = (uint64_t)a.dv * DK;
+    const bool zero = a.fresh && a.fresh[req];
+    float s[kScanRows];
+#pragma unroll
+    for (int r = 0; r < kScanRows; r++)
+        s[r] = zero ? 0.f : a.state[slot * a.slot_stride + h * per_head + (uint64_t)(r0 + r) * DK + j];
+    const uint32_t n_seg = (uint32_t)((t1 - t0 + seg - 1) / seg);
+    for (uint32_t p = 0; p < n_seg; p++) {
+        const uint64_t id = segment_id(ca, t0, req, p) * a.hv + h;
+#pragma unroll
+        for (int r = 0; r < kScanRows; r++) ca.s_in[id * per_head + (uint64_t)(r0 + r) * DK + j] = s[r];
+        if (p + 1 == n_seg) break;
+#pragma unroll
+        for (int r = 0; r < kScanRows; r++) reinterpret_cast<float*>(rows[r])[j] = s[r];
+        const float* m = ca.m_seg + id * (DK * DK) + j;
+#pragma unroll
+        for (int r = 0; r < kScanRows; r++) s[r] = ca.b_seg[id * per_head + (uint64_t)(r0 + r) * DK + j];
+        __syncthreads();
+#pragma unroll 8
+        for (int k = 0; k < DK / 4; k++) {
+            const float m0 = m[(4 * k) * DK], m1 = m[(4 * k + 1) * DK], m2 = m[(4 * k + 2) * DK], m3 = m[(4 * k + 3) * DK];
+#pragma unroll
+            for (int r = 0; r < kScanRows; r++) {
+                const float4 x = rows[r][k];
+                s[r] = fmaf(x.x, m0, fmaf(x.y, m1, fmaf(x.z, m2, fmaf(x.w, m3, s[r]))));
+            }
+        }
+        __syncthreads();
     }
 }
 

@@ -57,8 +57,10 @@ cudaError_t set_smem() {
 
 template <int DK, class T>
 cudaError_t set_chunk_smem() {
-    return cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)sizeof(rk::delta::ChunkSmem<DK, T>));
+    const int bytes = (int)sizeof(rk::delta::ChunkSmem<DK, T>);
+    if (cudaError_t e = cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+    if (cudaError_t e = cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+    return cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 // The current device's facts; the first call on a device looks them up and sets the kernels'
@@ -134,11 +136,48 @@ int32_t delta_args(const char* what, rk::delta::Args& a, const void* d_q, const 
     return BACKEND_OK;
 }
 
+uint64_t seg_floats(uint64_t hv, uint64_t dk, uint64_t dv) { return hv * dk * (2 * dv + dk); }   // b, s_in, M of a segment
+
+// Table blocks per segment, 0 = the requests are not cut.  Estimated time in chunk steps of one block alone
+// on its SM: co-resident blocks slow one another by about 0.4 of a step each, blocks past the
+// resident ones wait for a wave.  The transition pass has the key's rows beside the value's and, with
+// no outputs, steps of about 0.7; a scan step is about 0.1.  Only the requests' mean length is
+// known here.  16,384 tokens of one request, 8 heads of 128: 2.71 ms uncut.
+uint32_t segment_merge(const Device& d, const rk::delta::Args& a, uint32_t dk, uint32_t block, int resident, uint64_t work_bytes) {
+    const auto steps = [&](double blocks) {
+        const double k = blocks / d.sms, waves = std::ceil(blocks / (double)(d.sms * resident));
+        return waves * (1.0 + 0.4 * (std::max(1.0, std::min(k, (double)resident)) - 1.0));
+    };
+    const double slices = (double)ceil_div(a.dv, rk::delta::kVRows), both = (double)ceil_div(a.dv + dk, rk::delta::kVRows);
+    double best = 0.8 * (double)a.n_rows / rk::delta::kC / a.n * steps(a.n * (double)a.hv * slices);
+    uint32_t merge = 0;
+    for (uint32_t m = 1; (uint64_t)m * block * a.n <= a.n_rows; m *= 2) {
+        const uint64_t segs = a.n_rows / ((uint64_t)m * block) + a.n;
+        if (segs * seg_floats(a.hv, dk, a.dv) * 4 > work_bytes) continue;
+        const double chunks = (double)m * block / rk::delta::kC;
+        const double t = chunks * (0.7 * steps(segs * (double)a.hv * both) + steps(segs * (double)a.hv * slices)) + 0.1 * segs / a.n + 1.0;
+        if (t < best) best = t, merge = m;
+    }
+    return merge;
+}
+
 template <int DK, class T>
-int32_t launch_chunk(const rk::delta::ChunkArgs& ca, cudaStream_t st) {
+int32_t launch_chunk(const Device& d, rk::delta::ChunkArgs ca, uint32_t max_blocks, void* d_work, uint64_t work_bytes, cudaStream_t st) {
     using namespace rk::delta;
-    const dim3 grid((unsigned)ceil_div(ca.a.dv, kVRows), ca.a.hv, ca.a.n);
-    k_delta_chunk<DK, T, 0><<<grid, kCThreads, sizeof(ChunkSmem<DK, T>), st>>>(ca);
+    const unsigned slices = (unsigned)ceil_div(ca.a.dv, kVRows), smem = (unsigned)sizeof(ChunkSmem<DK, T>);
+    if (ca.blocks && d_work) ca.merge = segment_merge(d, ca.a, DK, ca.block, ChunkCfg<DK, T>::kMinBlocks, work_bytes);
+    else ca.merge = 0;
+    if (!ca.merge) {
+        k_delta_chunk<DK, T, 0><<<dim3(slices, ca.a.hv, ca.a.n), kCThreads, smem, st>>>(ca);
+    } else {
+        const uint64_t segs = ca.a.n_rows / ((uint64_t)ca.merge * ca.block) + ca.a.n;
+        ca.b_seg = static_cast<float*>(d_work);
+        ca.s_in = ca.b_seg + segs * ca.a.hv * ca.a.dv * DK;
+        ca.m_seg = ca.s_in + segs * ca.a.hv * ca.a.dv * DK;
+        k_delta_chunk<DK, T, 1><<<dim3((unsigned)ceil_div(ca.a.dv + DK, kVRows), ca.a.hv, max_blocks), kCThreads, smem, st>>>(ca);
+        k_delta_scan<DK><<<dim3((unsigned)ceil_div(ca.a.dv, kScanRows), ca.a.hv, ca.a.n), DK, 0, st>>>(ca);
+        k_delta_chunk<DK, T, 2><<<dim3(slices, ca.a.hv, max_blocks), kCThreads, smem, st>>>(ca);
+    }
     OP_CK(cudaGetLastError());
     return BACKEND_OK;
 }
@@ -321,6 +360,7 @@ int32_t redukt_b200_delta_chunk(const void* d_q, const void* d_k, const void* d_
         return rc;
     if (n_requests == 0) return BACKEND_OK;
     OP_REQUIRE(d_cu, "delta_chunk: NULL argument");
+    OP_REQUIRE(max_blocks <= 65535, "delta_chunk: %u table blocks (at most 65535: take a larger block)", max_blocks);
     OP_REQUIRE(!d_blocks || (block > 0 && block % 64 == 0 && (uint64_t)n_tokens / block + n_requests <= max_blocks),
                "delta_chunk: a block table needs a block of a multiple of 64 tokens and max_blocks of n_tokens / block + n_requests");
     OP_REQUIRE(!d_work || aligned(d_work, 256), "delta_chunk: the workspace is not 256-byte aligned");
@@ -329,9 +369,12 @@ int32_t redukt_b200_delta_chunk(const void* d_q, const void* d_k, const void* d_
     a.err = d->err;
     a.cu = d_cu;
     const cudaStream_t st = stream_of(cuda_stream);
-    rk::delta::ChunkArgs ca = {a, nullptr, 0, 1, nullptr, nullptr, nullptr};
-    if (dtype == REDUKT_DTYPE_F32) return d_key == 64 ? launch_chunk<64, float>(ca, st) : launch_chunk<128, float>(ca, st);
-    return d_key == 64 ? launch_chunk<64, __nv_bfloat16>(ca, st) : launch_chunk<128, __nv_bfloat16>(ca, st);
+    rk::delta::ChunkArgs ca = {a, d_blocks, block, 0, nullptr, nullptr, nullptr};
+    if (dtype == REDUKT_DTYPE_F32)
+        return d_key == 64 ? launch_chunk<64, float>(*d, ca, max_blocks, d_work, work_bytes, st)
+                           : launch_chunk<128, float>(*d, ca, max_blocks, d_work, work_bytes, st);
+    return d_key == 64 ? launch_chunk<64, __nv_bfloat16>(*d, ca, max_blocks, d_work, work_bytes, st)
+                       : launch_chunk<128, __nv_bfloat16>(*d, ca, max_blocks, d_work, work_bytes, st);
 }
 
 int32_t redukt_b200_quantize_tokens(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q,
@@ -346,8 +389,7 @@ int32_t redukt_b200_quantize_tokens(const void* d_x, int32_t dtype, uint32_t n_t
 }
 
 uint64_t redukt_b200_delta_work_bytes(uint32_t max_blocks, uint32_t n_v_heads, uint32_t d_key, uint32_t d_value) {
-    (void)max_blocks, (void)n_v_heads, (void)d_key, (void)d_value;
-    return 0;
+    return (uint64_t)max_blocks * seg_floats(n_v_heads, d_key, d_value) * sizeof(float);
 }
 
 uint64_t redukt_b200_w8a8_work_bytes(uint32_t n_tokens, uint32_t n_out, uint32_t k) {
