@@ -1,18 +1,20 @@
-// The gated delta rule over whole windows, 64 tokens at a time, on the warp-level tensor cores.
+// The gated delta rule over whole windows, 32 tokens at a time, on the warp-level tensor cores.
 //
 // With c_i the running sum of the log decays inside a chunk and S_0 the state before it:
 //   A_ij = b_i e^{c_i - c_j} k_i.k_j  (j < i),   (I + A) U = b (V - e^{c} K S_0^T)
 //   O = scale (e^{c} Q S_0^T + [e^{c_i - c_j} q_i.k_j]_{j <= i} U)
-//   S_64 = e^{c_64} S_0 + sum_j e^{c_64 - c_j} u_j k_j^T
+//   S_32 = e^{c_32} S_0 + sum_j e^{c_32 - c_j} u_j k_j^T
 // Every exponent is a difference c_i - c_j with j <= i, so nothing overflows however strong the decay
 // is.  c is summed in 64 bits and kept as two floats (times log2 e).
 //
-// Split: one block of 4 warps per (request, value head, 64 state rows); a state row depends on no
-// other, so a warp keeps 16 of them in registers as mma accumulators for the whole request, and every
-// product of the chain (X = S K^T, the solve, O, the update) turns accumulators straight into the next
-// product's A operand.  Only K, Q, A and P pass through shared memory.  The triangular system is
-// solved by 16-token blocks (their 16 x 16 diagonal blocks are inverted by substitution, the rest is
-// subtracted), which stays accurate where the whole inverse would not (equal keys).
+// Split: a state row depends on no other, so a warp keeps 16 of them in registers as mma accumulators for
+// the whole request, and every product of the chain (X = S K^T, the solve, O, the update) turns
+// accumulators straight into the next product's A operand.  Only K, Q and what derives from them
+// passes through shared memory.  The triangular system is solved by 16-token blocks: with D_i the
+// inverse of a diagonal block of I + A and B_ij = D_i A_ij, both by forward substitution,
+//   U_0 = D_0 R_0,  U_1 = D_1 R_1 - B_10 U_0,
+// which stays accurate where the whole inverse would not (equal keys) and leaves one product on the
+// chain from U_0 to U_1.
 //
 // Precision: an f32 operand is split into two f16 planes hi + lo after scaling its row by a power of
 // two that puts the row's largest value in [2^14, 2^15): 22 bits of every value down to 2^-28 of that
@@ -27,27 +29,25 @@
 namespace rk {
 namespace delta {
 
-constexpr int kC = 64;              // tokens per chunk
+constexpr int kC = 32;              // tokens per chunk
+constexpr int kNB = kC / 16;        // 16-token blocks of a chunk
 constexpr int kCWarps = 4;
 constexpr int kCThreads = kCWarps * 32;
 constexpr int kVRows = 16 * kCWarps;  // state rows per block
 
-// Lower triangle of a 64 x 64 matrix by strips of 16 rows: strip r is 16 (r + 1) wide; a row's stride is
-// an odd number of 16-byte units, so ldmatrix reads 8 rows without a bank conflict.
-constexpr int kStripHalves = 16 * (24 + 40 + 56 + 72);
-__device__ __forceinline__ int strip_at(int row, int col) {
-    const int r = row >> 4;
-    return 16 * (8 * r + 8 * r * (r + 1)) + (row & 15) * (16 * r + 24) + col;
-}
-
-constexpr int kDiagLd = 20;         // rows of 16 floats on 16 bytes, two columns apart in other banks
+// Lower triangle of a kC x kC matrix in two planes, by strips of 16 rows: strip r is 16 (r + 1) wide; a
+// row's stride is an odd number of 16-byte units, so ldmatrix reads 8 rows without a bank conflict.
+// A strip's low plane follows its high one.
+constexpr int kStripHalves = 2 * 16 * (24 + 40);
+__host__ __device__ constexpr int strip_ld(int r) { return 16 * r + 24; }
+__host__ __device__ constexpr int strip_base(int r) { return 2 * 16 * (8 * r + 8 * r * (r + 1)); }
 
 template <int DK, class T>
 struct ChunkCfg {
     static constexpr bool kF32 = sizeof(T) == 4;
     static constexpr int KP = kF32 ? 2 : 1;     // planes of k and q
     static constexpr int LD = DK + 8;           // halves per row of a plane
-    static constexpr int kMinBlocks = DK == 64 ? 3 : 2;
+    static constexpr int kMinBlocks = DK == 64 ? 4 : 3;
 };
 
 template <int DK, class T>
@@ -55,18 +55,16 @@ struct alignas(16) ChunkSmem {
     using Cfg = ChunkCfg<DK, T>;
     __half k[Cfg::KP][kC * Cfg::LD];
     __half q[Cfg::KP][kC * Cfg::LD];
-    __half m[2][kStripHalves];          // A below the diagonal blocks, their inverses on them
-    __half p[2][kStripHalves];
-    float diag[kCWarps][16 * kDiagLd];  // a diagonal block, transposed: [column][row]
+    __half m[kStripHalves];             // B below the diagonal blocks, D on them; before that, A in f32
+    __half p[kStripHalves];
     float sk[kC], sq[kC];               // row scales of the planes, norms folded in
     float chi[kC], clo[kC];             // c * log2(e) in two floats
     float beta[kC];
+    float ee[kC];                       // e^{c_i}
     float ak[kC], cq[kC], wk[kC];       // factors of X, O and the update, per token
-    float rf[kC];                       // e^{c_i - c_ref}, ref = the token before i's strip
-    float cf[3][kC];                    // strip r + 1: e^{c_ref - c_j} times the key's scale
-    float ascale[4][kC], pscale[4][kC]; // scales of a row of each 16 x 16 block of A and P
-    float dblk[kCWarps];                // scale of each inverted block
-    float gamma;
+    float rf[16], cf[16];               // block (1, 0): e^{c_i - c_15} of its rows, e^{c_15 - c_j} of its columns
+    float pscale[kNB][kC];              // scale of a row of each 16 x 16 block of P
+    float dscale[kNB], bscale;          // scales of D and B
 };
 
 struct ChunkArgs {
@@ -186,7 +184,7 @@ struct RowLoad {
     }
 };
 
-// Four rows of each 8-lane group: r, r + 4, r + 8, r + 12 of the warp's 16.
+// Four rows of each 8-lane group: row, row + 4, row + 8, row + 12.
 template <int DK, class T>
 __device__ __forceinline__ void put_rows(RowLoad<DK, T> (&x)[4], __half* hi, __half* lo, int ld, float* scale, int row, int len, bool l2norm, int l) {
     float m[4], ss[4], s[4], inv[4];
@@ -214,114 +212,98 @@ __device__ __forceinline__ void put_rows(RowLoad<DK, T> (&x)[4], __half* hi, __h
     }
 }
 
-// Fills the chunk's shared operands: planes and scales of k and q, decay factors, A, its inverted
-// diagonal blocks, and P.  All warps; ends with a barrier.
+// A barrier of the four warps that prepare a chunk.
+__device__ __forceinline__ void prep_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kCThreads) : "memory"); }
+
+// Where A's value (row of the strip, column) waits for the substitution: by columns of 16 floats, their
+// four 16-byte parts swapped so that the mma layout's stores meet two to a bank at most.
+__device__ __forceinline__ int wait_at(int row, int col) { return col * 16 + ((((row >> 2) ^ (col >> 1)) & 3) << 2) + (row & 3); }
+
+// Fills the chunk's shared operands: planes and scales of k and q, decay factors, D and B, and P.  Run by
+// four warps (`warp` 0..3); the caller's barrier publishes the last writes.
 template <int DK, class T, bool kOut>
 __device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& a, uint64_t t0, int len, uint32_t h, uint32_t hq,
-                                              bool wide) {
+                                              bool wide, int warp) {
     using Cfg = ChunkCfg<DK, T>;
     constexpr int LD = Cfg::LD, KP = Cfg::KP;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane >> 3, l = lane & 7, g = lane >> 2, t = lane & 3;
-    {
-        const T* kp = (const T*)a.k + t0 * a.ld_k + (uint64_t)hq * DK;
-        const T* qp = (const T*)a.q + t0 * a.ld_q + (uint64_t)hq * DK;
-        const int row = warp * 16 + grp;
-        RowLoad<DK, T> rk[4], rq[4];
+    const int lane = threadIdx.x & 31, grp = lane >> 3, l = lane & 7, g = lane >> 2, t = lane & 3;
+    const bool key = warp < 2;                    // warps 0 and 1 bring k's rows, 2 and 3 q's
+    const int row = (warp & 1) * 16 + grp;
+    RowLoad<DK, T> rows[4];
+    if (kOut || key) {
+        const T* p = key ? (const T*)a.k + t0 * a.ld_k + (uint64_t)hq * DK : (const T*)a.q + t0 * a.ld_q + (uint64_t)hq * DK;
+        const uint64_t ld = key ? a.ld_k : a.ld_q;
 #pragma unroll
         for (int i = 0; i < 4; i++) {   // rows past the end read the last one and are cleared
             const uint32_t r = min(row + 4 * i, len - 1);
-            if (wide) {
-                rk[i].load(kp + r * a.ld_k, l);
-                if (kOut) rq[i].load(qp + r * a.ld_q, l);
-            } else {
-                rk[i].load_single(kp + r * a.ld_k, l);
-                if (kOut) rq[i].load_single(qp + r * a.ld_q, l);
-            }
+            if (wide) rows[i].load(p + r * ld, l);
+            else rows[i].load_single(p + r * ld, l);
         }
-        if (warp == 0) {   // tokens 2 lane, 2 lane + 1
-            double c0 = 0.0, c1 = 0.0;
-            float b0 = 0.f, b1 = 0.f;
-            const int i0 = 2 * lane;
-            if (i0 < len) {
-                const float x = a.g[(t0 + i0) * a.ld_g + h];
-                c0 = x < -1000.f ? -1000.0 : (double)x;   // e^-1000 is 0 in f32; -inf - -inf would be NaN
-                b0 = a.beta[(t0 + i0) * a.ld_g + h];
-            }
-            if (i0 + 1 < len) {
-                const float x = a.g[(t0 + i0 + 1) * a.ld_g + h];
-                c1 = x < -1000.f ? -1000.0 : (double)x;
-                b1 = a.beta[(t0 + i0 + 1) * a.ld_g + h];
-            }
-            double s = c0 + c1;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xFFFFFFFFu, s, o);
-                if (lane >= o) s += y;
-            }
-            const double e1 = s * 1.4426950408889634, e0 = (s - c1) * 1.4426950408889634;   // log2(e)
-            sm.chi[i0] = (float)e0;
-            sm.clo[i0] = (float)(e0 - (double)(float)e0);
-            sm.chi[i0 + 1] = (float)e1;
-            sm.clo[i0 + 1] = (float)(e1 - (double)(float)e1);
-            sm.beta[i0] = b0;
-            sm.beta[i0 + 1] = b1;
-        }
-        put_rows<DK, T>(rk, sm.k[0], sm.k[KP - 1], LD, sm.sk, row, len, a.l2norm, l);
-        if (kOut) put_rows<DK, T>(rq, sm.q[0], sm.q[KP - 1], LD, sm.sq, row, len, a.l2norm, l);
     }
-    __syncthreads();
-    if (threadIdx.x < kC) {
-        const int i = threadIdx.x, ref = (i & ~15) - 1;
-        const float c = sm.chi[i] + sm.clo[i], e = exp2f(c);
-        const float w = exp2f((sm.chi[kC - 1] - sm.chi[i]) + (sm.clo[kC - 1] - sm.clo[i]));
-        sm.ak[i] = e * sm.sk[i];
-        sm.wk[i] = w * sm.sk[i];
-        if (kOut) sm.cq[i] = a.scale * e * sm.sq[i];
-        if (i == kC - 1) sm.gamma = e;
-        sm.rf[i] = ref < 0 ? 1.f : exp2f((sm.chi[i] - sm.chi[max(ref, 0)]) + (sm.clo[i] - sm.clo[max(ref, 0)]));
+    if (warp != 1) {   // the warps have c of token `lane`; each writes its share of the factors
+        double s = 0.0;
+        if (lane < len) {
+            const float x = a.g[(t0 + lane) * a.ld_g + h];
+            s = x < -1000.f ? -1000.0 : (double)x;   // e^-1000 is 0 in f32; -inf - -inf would be NaN
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xFFFFFFFFu, s, o);
+            if (lane >= o) s += y;
+        }
+        const double e = s * 1.4426950408889634;   // log2(e)
+        const float hi = (float)e, lo = (float)(e - (double)hi);
+        if (warp == 0) {
+            sm.chi[lane] = hi;
+            sm.clo[lane] = lo;
+            sm.ee[lane] = exp2f(hi + lo);
+        } else if (warp == 2) {
+            const float he = __shfl_sync(0xFFFFFFFFu, hi, kC - 1), le = __shfl_sync(0xFFFFFFFFu, lo, kC - 1);
+            sm.wk[lane] = exp2f((he - hi) + (le - lo));
+        } else {
+            const float hr = __shfl_sync(0xFFFFFFFFu, hi, 15), lr = __shfl_sync(0xFFFFFFFFu, lo, 15);
+            const float x = exp2f(lane < 16 ? (hr - hi) + (lr - lo) : (hi - hr) + (lo - lr));
+            (lane < 16 ? sm.cf : sm.rf)[lane & 15] = x;
+        }
     } else {
-        const int j = threadIdx.x - kC;
-#pragma unroll
-        for (int r = 1; r < 4; r++)
-            if (j < 16 * r) sm.cf[r - 1][j] = sm.sk[j] * exp2f((sm.chi[16 * r - 1] - sm.chi[j]) + (sm.clo[16 * r - 1] - sm.clo[j]));
+        sm.beta[lane] = lane < len ? a.beta[(t0 + lane) * a.ld_g + h] : 0.f;
     }
-    // Strip r of a product is rows 16 r .. 16 r + 15 against tokens 0 .. 16 r + 15.  Warp w does strip w of
-    // K K^T and strip 3 - w of Q K^T, five 16 x 16 blocks for every warp: slot 0 the diagonal block of the
-    // first, slot 1 that of the second, slots 2-4 the blocks beside them.
-    const int rg = warp, rh = kCWarps - 1 - warp;
-    float acc[5][2][4];
+    if (kOut || key)
+        put_rows<DK, T>(rows, key ? sm.k[0] : sm.q[0], key ? sm.k[KP - 1] : sm.q[KP - 1], LD, key ? sm.sk : sm.sq, row, len, a.l2norm, l);
+    prep_sync();
+    if (warp == 3) {
+        sm.ak[lane] = sm.ee[lane] * sm.sk[lane];
+        sm.wk[lane] *= sm.sk[lane];
+        if (kOut) sm.cq[lane] = a.scale * sm.ee[lane] * sm.sq[lane];
+    }
+    // Strip r of a product is rows 16 r .. 16 r + 15 against tokens 0 .. 16 r + 15, slot s of it the tokens 16 s ..
+    // Warps 0 and 2 do strips 1 and 0 of K K^T, warps 1 and 3 those of Q K^T.
+    const bool gram = (warp & 1) == 0;
+    const int r = 1 - (warp >> 1);
+    if (!kOut && !gram) return;
+    float acc[2][2][4];
 #pragma unroll
-    for (int s = 0; s < 5; s++)
+    for (int s = 0; s < 2; s++)
 #pragma unroll
         for (int c = 0; c < 4; c++) acc[s][0][c] = acc[s][1][c] = 0.f;
     {
-        const int arow = (lane & 7) + ((lane >> 3) & 1) * 8, acol = (lane >> 4) * 8;
-        const int brow = (lane & 7) + (lane >> 4) * 8, bcol = ((lane >> 3) & 1) * 8;
+        const int aoff = (16 * r + (lane & 7) + ((lane >> 3) & 1) * 8) * LD + (lane >> 4) * 8;
+        const int boff = ((lane & 7) + (lane >> 4) * 8) * LD + ((lane >> 3) & 1) * 8;
+        const __half* ah = (gram ? sm.k[0] : sm.q[0]) + aoff;
+        const __half* al = (gram ? sm.k[KP - 1] : sm.q[KP - 1]) + aoff;
 #pragma unroll
         for (int ks = 0; ks < DK / 16; ks++) {
-            uint32_t fk[4], fkl[4], fq[4], fql[4];
-            ldsm4(fk, &sm.k[0][(16 * rg + arow) * LD + ks * 16 + acol]);
-            if (KP == 2) ldsm4(fkl, &sm.k[KP - 1][(16 * rg + arow) * LD + ks * 16 + acol]);
-            if (kOut) {
-                ldsm4(fq, &sm.q[0][(16 * rh + arow) * LD + ks * 16 + acol]);
-                if (KP == 2) ldsm4(fql, &sm.q[KP - 1][(16 * rh + arow) * LD + ks * 16 + acol]);
-            }
+            uint32_t fa[4], fl[4];
+            ldsm4(fa, ah + ks * 16);
+            if (KP == 2) ldsm4(fl, al + ks * 16);
 #pragma unroll
-            for (int s = 0; s < 5; s++) {
-                const bool key = s == 0 || (s > 1 && s - 2 < warp);
-                if (!kOut && !key) continue;
-                const int nb = s == 0 ? rg : s == 1 ? rh : s - 2 < warp ? s - 2 : s - 2 - warp;
-                uint32_t fa[4], fl[4], fb[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    fa[c] = !kOut || key ? fk[c] : fq[c];
-                    if (KP == 2) fl[c] = !kOut || key ? fkl[c] : fql[c];
-                }
-                const int off = (nb * 16 + brow) * LD + ks * 16 + bcol;
-                ldsm4(fb, &sm.k[0][off]);
+            for (int s = 0; s < 2; s++) {
+                if (s > r) continue;
+                uint32_t fb[4];
+                ldsm4(fb, &sm.k[0][s * 16 * LD + boff + ks * 16]);
                 if (KP == 2) {
                     uint32_t fw[4];
-                    ldsm4(fw, &sm.k[KP - 1][off]);
+                    ldsm4(fw, &sm.k[KP - 1][s * 16 * LD + boff + ks * 16]);
                     mma_f16(acc[s][0], fa, fw[0], fw[1]);
                     mma_f16(acc[s][1], fa, fw[2], fw[3]);
                     mma_f16(acc[s][0], fl, fb[0], fb[1]);
@@ -332,118 +314,104 @@ __device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& 
             }
         }
     }
-    __syncthreads();   // the factors below
-    {
-        const int ig = 16 * rg + g, ih = 16 * rh + g;
-        const float kg0 = sm.beta[ig] * sm.sk[ig], kg1 = sm.beta[ig + 8] * sm.sk[ig + 8];
-        const float kh0 = kOut ? a.scale * sm.sq[ih] : 0.f, kh1 = kOut ? a.scale * sm.sq[ih + 8] : 0.f;
-        // diagonal blocks: every pair's own exponent (column 8 n + 2 t + c of the block, rows g and g + 8)
+    const int ld = strip_ld(r);
+    __half* hi = (gram ? sm.m : sm.p) + strip_base(r);
+    __half* lo = hi + 16 * ld;
+    float* wait = reinterpret_cast<float*>(hi);   // 1,024 (r + 1) of the strip's bytes
+    const int i0 = 16 * r + g;
+    const float k0 = gram ? sm.beta[i0] * sm.sk[i0] : a.scale * sm.sq[i0];
+    const float k1 = gram ? sm.beta[i0 + 8] * sm.sk[i0 + 8] : a.scale * sm.sq[i0 + 8];
+    const float ch0 = sm.chi[i0], cl0 = sm.clo[i0], ch1 = sm.chi[i0 + 8], cl1 = sm.clo[i0 + 8];
 #pragma unroll
-        for (int s = 0; s < (kOut ? 2 : 1); s++) {
-            const int i0 = s ? ih : ig, base = 16 * (s ? rh : rg);
-            const float r0 = s ? kh0 : kg0, r1 = s ? kh1 : kg1;
-            const float ch0 = sm.chi[i0], cl0 = sm.clo[i0], ch1 = sm.chi[i0 + 8], cl1 = sm.clo[i0 + 8];
+    for (int s = 0; s < 2; s++) {   // columns 16 s + 8 n + 2 t + c; s == r is the diagonal block
+        if (s > r) continue;
+        const bool diag = s == r;
+        const float f0 = k0 * sm.rf[g], f1 = k1 * sm.rf[g + 8];
+        float m0 = 0.f, m1 = 0.f;
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+        for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const int jj = 8 * n + 2 * t + c, j = base + jj;
-                    const float kj = sm.sk[j], h = sm.chi[j], w = sm.clo[j];
-                    const float e0 = exp2f((ch0 - h) + (cl0 - w)), e1 = exp2f((ch1 - h) + (cl1 - w));
-                    const bool in0 = s ? jj <= g : jj < g, in1 = s ? jj <= g + 8 : jj < g + 8;
-                    acc[s][n][c] = in0 ? acc[s][n][c] * (r0 * kj) * e0 : 0.f;
-                    acc[s][n][2 + c] = in1 ? acc[s][n][2 + c] * (r1 * kj) * e1 : 0.f;
-                    if (s == 0) {
-                        sm.diag[warp][jj * kDiagLd + g] = acc[0][n][c];
-                        sm.diag[warp][jj * kDiagLd + g + 8] = acc[0][n][2 + c];
-                    }
+            for (int c = 0; c < 2; c++) {
+                const int jj = 8 * n + 2 * t + c, j = 16 * s + jj;
+                const float kj = sm.sk[j];
+                if (diag) {   // every pair's own exponent
+                    const float hj = sm.chi[j], lj = sm.clo[j];
+                    const float e0 = exp2f((ch0 - hj) + (cl0 - lj)), e1 = exp2f((ch1 - hj) + (cl1 - lj));
+                    acc[s][n][c] = jj < g + !gram ? acc[s][n][c] * (k0 * kj) * e0 : 0.f;
+                    acc[s][n][2 + c] = jj < g + 8 + !gram ? acc[s][n][2 + c] * (k1 * kj) * e1 : 0.f;
+                } else {      // a factor per row and one per column
+                    const float f = sm.cf[jj] * kj;
+                    acc[s][n][c] *= f0 * f;
+                    acc[s][n][2 + c] *= f1 * f;
                 }
+                if (gram) {
+                    wait[wait_at(g, j)] = acc[s][n][c];
+                    wait[wait_at(g + 8, j)] = acc[s][n][2 + c];
+                }
+                m0 = amax(m0, acc[s][n][c]);
+                m1 = amax(m1, acc[s][n][2 + c]);
+            }
+        if (gram) continue;
+        float v0, v1;
+        const float p0 = row_pow(quad_max(m0), v0), p1 = row_pow(quad_max(m1), v1);
+        if (t == 0) {
+            sm.pscale[s][i0] = v0;
+            sm.pscale[s][i0 + 8] = v1;
         }
-        // the blocks beside them: a factor per row and one per column
-        const float fg0 = kg0 * sm.rf[ig], fg1 = kg1 * sm.rf[ig + 8], fh0 = kh0 * sm.rf[ih], fh1 = kh1 * sm.rf[ih + 8];
 #pragma unroll
-        for (int s = 1; s < 5; s++) {
-            const bool key = s > 1 && s - 2 < warp;
-            if (!kOut && !key) continue;
-            const int nb = s == 1 ? rh : key ? s - 2 : s - 2 - warp;
-            const int r = key ? rg : rh, i0 = 16 * r + g;
-            if (s > 1) {
-                const float* cf = sm.cf[r - 1] + 16 * nb + 2 * t;
-                const float r0 = key ? fg0 : fh0, r1 = key ? fg1 : fh1;
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        acc[s][n][c] *= r0 * cf[8 * n + c];
-                        acc[s][n][2 + c] *= r1 * cf[8 * n + c];
-                    }
-            }
-            float m0 = 0.f, m1 = 0.f, v0, v1;
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    m0 = amax(m0, acc[s][n][c]);
-                    m1 = amax(m1, acc[s][n][2 + c]);
-                }
-            const float p0 = row_pow(quad_max(m0), v0), p1 = row_pow(quad_max(m1), v1);
-            float* sc = key ? sm.ascale[nb] : sm.pscale[nb];
-            if (t == 0) {
-                sc[i0] = v0;
-                sc[i0 + 8] = v1;
-            }
-            __half* hi = key ? sm.m[0] : sm.p[0];
-            __half* lo = key ? sm.m[1] : sm.p[1];
-            const int at = strip_at(i0, 16 * nb + 2 * t), down = 8 * (16 * r + 24);
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                uint32_t x, y;
-                split2(acc[s][n][0] * p0, acc[s][n][1] * p0, x, y);
-                *reinterpret_cast<uint32_t*>(hi + at + 8 * n) = x;
-                *reinterpret_cast<uint32_t*>(lo + at + 8 * n) = y;
-                split2(acc[s][n][2] * p1, acc[s][n][3] * p1, x, y);
-                *reinterpret_cast<uint32_t*>(hi + at + down + 8 * n) = x;
-                *reinterpret_cast<uint32_t*>(lo + at + down + 8 * n) = y;
-            }
+        for (int n = 0; n < 2; n++) {
+            const int at = g * ld + 16 * s + 8 * n + 2 * t;
+            uint32_t x, y;
+            split2(acc[s][n][0] * p0, acc[s][n][1] * p0, x, y);
+            *reinterpret_cast<uint32_t*>(hi + at) = x;
+            *reinterpret_cast<uint32_t*>(lo + at) = y;
+            split2(acc[s][n][2] * p1, acc[s][n][3] * p1, x, y);
+            *reinterpret_cast<uint32_t*>(hi + at + 8 * ld) = x;
+            *reinterpret_cast<uint32_t*>(lo + at + 8 * ld) = y;
         }
     }
+    if (!gram) return;
     __syncwarp();
-    {   // (I + A_ww)^-1 by forward substitution, lane c < 16 its column c (lanes 16.. repeat it)
-        const int c = lane & 15;
-        const float* at = sm.diag[warp];
-        float x[16];
+    // forward substitution with the unit lower diagonal block: lane c solves for column c of
+    // [A beside the block, I], 16 (r + 1) of them
+    const int unit = 16 * r;
+    float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = i == c ? 1.f : 0.f;
-#pragma unroll
-        for (int j = 0; j < 15; j++) {
-            float col[16];
-#pragma unroll
-            for (int i = (j + 1) & ~3; i < 16; i += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(at + j * kDiagLd + i);
-                col[i] = f.x, col[i + 1] = f.y, col[i + 2] = f.z, col[i + 3] = f.w;
-            }
-#pragma unroll
-            for (int i = j + 1; i < 16; i++) x[i] = fmaf(-col[i], x[j], x[i]);
-        }
-        float m = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; i++) m = amax(m, x[i]);
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        float inv;
-        const float s = row_pow(m, inv);
-        if (lane == 0) sm.dblk[warp] = inv;
-        if (lane < 16)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float y = x[i] * s;
-                const __half hh = __float2half_rn(y);
-                const int at0 = strip_at(16 * warp + i, 16 * warp + c);
-                sm.m[0][at0] = hh;
-                sm.m[1][at0] = __float2half_rn(y - __half2float(hh));
-            }
+    for (int i = 0; i < 16; i += 4) {
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (lane < unit) f = *reinterpret_cast<const float4*>(wait + wait_at(i, lane));
+        x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
     }
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; i++) x[i] = lane == unit + i ? 1.f : x[i];
+#pragma unroll
+    for (int j = 0; j < 15; j++) {
+        float col[16];
+#pragma unroll
+        for (int i = (j + 1) & ~3; i < 16; i += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(wait + wait_at(i, unit + j));
+            col[i] = f.x, col[i + 1] = f.y, col[i + 2] = f.z, col[i + 3] = f.w;
+        }
+#pragma unroll
+        for (int i = j + 1; i < 16; i++) x[i] = fmaf(-col[i], x[j], x[i]);
+    }
+    __syncwarp();   // the strip's planes take the place of A
+    float m = 0.f, inv;
+#pragma unroll
+    for (int i = 0; i < 16; i++) m = amax(m, x[i]);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));   // per 16 columns: B and D apart
+    const float s = row_pow(m, inv);
+    if (lane == 0 && r) sm.bscale = inv;
+    if (lane == unit) sm.dscale[r] = inv;
+    if (lane < 16 * (r + 1))
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float y = x[i] * s;
+            const __half hh = __float2half_rn(y);
+            hi[i * ld + lane] = hh;
+            lo[i * ld + lane] = __float2half_rn(y - __half2float(hh));
+        }
 }
 
 // f32 accumulators of one 16-column group (two tiles) -> A operand planes, rows scaled; the inverse
@@ -464,18 +432,200 @@ __device__ __forceinline__ void to_planes(const float (&x)[4], const float (&y)[
 
 // d0, d1 (16 columns) += planes x a 16 x 16 block of a strip matrix (rows i = columns of the result)
 __device__ __forceinline__ void mma_block(float (&d0)[4], float (&d1)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4],
-                                          const __half* bhi, const __half* blo, int ib, int jb, int lane) {
-    const int row = 16 * ib + (lane & 7) + (lane >> 4) * 8, col = 16 * jb + ((lane >> 3) & 1) * 8;
-    const int at = strip_at(row, col);
+                                          const __half* strips, int ib, int jb, int lane) {
+    const __half* at = strips + strip_base(ib) + ((lane & 7) + (lane >> 4) * 8) * strip_ld(ib) + 16 * jb + ((lane >> 3) & 1) * 8;
     uint32_t b[4], w[4];
-    ldsm4(w, blo + at);
+    ldsm4(w, at + 16 * strip_ld(ib));
+    ldsm4(b, at);
     mma_f16(d0, hi, w[0], w[1]);
     mma_f16(d1, hi, w[2], w[3]);
-    ldsm4(b, bhi + at);
     mma_f16(d0, lo, b[0], b[1]);
     mma_f16(d1, lo, b[2], b[3]);
     mma_f16(d0, hi, b[0], b[1]);
     mma_f16(d1, hi, b[2], b[3]);
+}
+
+// One chunk's step of 16 state rows, by one warp: S (rows row0 + g and + 8, columns 8 n + 2 t, + 1) to the
+// state after it, with outputs where kOut.  vp and op: v and out at (row 0, this thread's first state row).
+template <int DK, class T, bool kOut>
+__device__ __forceinline__ void consume_chunk(const ChunkSmem<DK, T>& sm, float (&S)[DK / 8][4], const Args& a, const T* vp, T* op,
+                                              uint64_t at, int len, bool ident) {
+    using Cfg = ChunkCfg<DK, T>;
+    constexpr int LD = Cfg::LD, KP = Cfg::KP, NT = DK / 8;
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    // X = S K^T and O = S Q^T over the chunk; V meanwhile
+    T V[kC / 8][4];
+#pragma unroll
+    for (int n = 0; n < kC / 8; n++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const int i = 8 * n + 2 * t + (c & 1);
+            V[n][c] = (i < len && !ident) ? vp[(at + i) * a.ld_v + (c >> 1) * 8] : T(0.f);
+        }
+    float X[kC / 8][4], O[kC / 8][4];
+#pragma unroll
+    for (int n = 0; n < kC / 8; n++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) X[n][c] = O[n][c] = 0.f;
+    {
+        float m0 = 0.f, m1 = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            m0 = amax(amax(m0, S[n][0]), S[n][1]);
+            m1 = amax(amax(m1, S[n][2]), S[n][3]);
+        }
+        float sv0, sv1;
+        const float p0 = row_pow(quad_max(m0), sv0), p1 = row_pow(quad_max(m1), sv1);
+        const int brow = (lane & 7) + (lane >> 4) * 8, bcol = ((lane >> 3) & 1) * 8;
+#pragma unroll
+        for (int ks = 0; ks < DK / 16; ks++) {
+            uint32_t hi[4], lo[4];
+            split2(S[2 * ks][0] * p0, S[2 * ks][1] * p0, hi[0], lo[0]);
+            split2(S[2 * ks][2] * p1, S[2 * ks][3] * p1, hi[1], lo[1]);
+            split2(S[2 * ks + 1][0] * p0, S[2 * ks + 1][1] * p0, hi[2], lo[2]);
+            split2(S[2 * ks + 1][2] * p1, S[2 * ks + 1][3] * p1, hi[3], lo[3]);
+#pragma unroll
+            for (int nn = 0; nn < kNB; nn++) {
+                const int off = (nn * 16 + brow) * LD + ks * 16 + bcol;
+                uint32_t b[4];
+                if (KP == 2) {
+                    ldsm4(b, &sm.k[KP - 1][off]);
+                    mma_f16(X[2 * nn], hi, b[0], b[1]);
+                    mma_f16(X[2 * nn + 1], hi, b[2], b[3]);
+                }
+                ldsm4(b, &sm.k[0][off]);
+                mma_f16(X[2 * nn], lo, b[0], b[1]);
+                mma_f16(X[2 * nn + 1], lo, b[2], b[3]);
+                mma_f16(X[2 * nn], hi, b[0], b[1]);
+                mma_f16(X[2 * nn + 1], hi, b[2], b[3]);
+                if (kOut) {
+                    if (KP == 2) {
+                        ldsm4(b, &sm.q[KP - 1][off]);
+                        mma_f16(O[2 * nn], hi, b[0], b[1]);
+                        mma_f16(O[2 * nn + 1], hi, b[2], b[3]);
+                    }
+                    ldsm4(b, &sm.q[0][off]);
+                    mma_f16(O[2 * nn], lo, b[0], b[1]);
+                    mma_f16(O[2 * nn + 1], lo, b[2], b[3]);
+                    mma_f16(O[2 * nn], hi, b[0], b[1]);
+                    mma_f16(O[2 * nn + 1], hi, b[2], b[3]);
+                }
+            }
+        }
+        // right-hand side R = b (V - e^c X), and the state's part of the output
+#pragma unroll
+        for (int n = 0; n < kC / 8; n++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int i = 8 * n + 2 * t + (c & 1);
+                const float sv = c < 2 ? sv0 : sv1;
+                X[n][c] = sm.beta[i] * (to_f32(V[n][c]) - sm.ak[i] * (sv * X[n][c]));
+                if (kOut) O[n][c] = sm.cq[i] * (sv * O[n][c]);
+            }
+    }
+    // U in the place of R; O_i += P_ij U_j
+    uint32_t uh[kNB][4], ul[kNB][4];
+#pragma unroll
+    for (int i = 0; i < kNB; i++) {
+        float inv[2], d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+        to_planes(X[2 * i], X[2 * i + 1], uh[i], ul[i], inv);
+        mma_block(d0, d1, uh[i], ul[i], sm.m, i, i, lane);
+        const float db = sm.dscale[i];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            X[2 * i][c] = d0[c] * (db * inv[c >> 1]);
+            X[2 * i + 1][c] = d1[c] * (db * inv[c >> 1]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kNB; j++) {
+        float us[2];
+        to_planes(X[2 * j], X[2 * j + 1], uh[j], ul[j], us);
+#pragma unroll
+        for (int i = j + 1; i < kNB; i++) {
+            float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_block(d0, d1, uh[j], ul[j], sm.m, i, j, lane);
+            const float b = -sm.bscale;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                X[2 * i][c] = fmaf(b * us[c >> 1], d0[c], X[2 * i][c]);
+                X[2 * i + 1][c] = fmaf(b * us[c >> 1], d1[c], X[2 * i + 1][c]);
+            }
+        }
+        if (kOut) {
+#pragma unroll
+            for (int i = j; i < kNB; i++) {
+                float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_block(d0, d1, uh[j], ul[j], sm.p, i, j, lane);
+                const float* ps = &sm.pscale[j][16 * i + 2 * t];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    O[2 * i][c] = fmaf(ps[c & 1] * us[c >> 1], d0[c], O[2 * i][c]);
+                    O[2 * i + 1][c] = fmaf(ps[8 + (c & 1)] * us[c >> 1], d1[c], O[2 * i + 1][c]);
+                }
+            }
+        }
+    }
+    if (kOut) {
+#pragma unroll
+        for (int n = 0; n < kC / 8; n++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int i = 8 * n + 2 * t + (c & 1);
+                if (i < len) put(op + (at + i) * a.ld_o + (c >> 1) * 8, O[n][c]);
+            }
+    }
+    // S = e^{c_32} S + sum_j (w_j u_j) k_j^T
+    float n0 = 0.f, n1 = 0.f;
+#pragma unroll
+    for (int n = 0; n < kC / 8; n++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const float w = sm.wk[8 * n + 2 * t + c];
+            X[n][c] *= w;
+            X[n][2 + c] *= w;
+            n0 = amax(n0, X[n][c]);
+            n1 = amax(n1, X[n][2 + c]);
+        }
+    float iv0, iv1;
+    const float q0 = row_pow(quad_max(n0), iv0), q1 = row_pow(quad_max(n1), iv1);
+#pragma unroll
+    for (int jb = 0; jb < kNB; jb++) {
+        split2(X[2 * jb][0] * q0, X[2 * jb][1] * q0, uh[jb][0], ul[jb][0]);
+        split2(X[2 * jb][2] * q1, X[2 * jb][3] * q1, uh[jb][1], ul[jb][1]);
+        split2(X[2 * jb + 1][0] * q0, X[2 * jb + 1][1] * q0, uh[jb][2], ul[jb][2]);
+        split2(X[2 * jb + 1][2] * q1, X[2 * jb + 1][3] * q1, uh[jb][3], ul[jb][3]);
+    }
+    const float gamma = sm.ee[kC - 1];
+    const int trow = (lane & 7) + ((lane >> 3) & 1) * 8, tcol = (lane >> 4) * 8;
+#pragma unroll
+    for (int nn = 0; nn < NT / 2; nn++) {
+        float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t b[kNB][4];
+#pragma unroll
+        for (int jb = 0; jb < kNB; jb++) {
+            const int off = (16 * jb + trow) * LD + nn * 16 + tcol;
+            if (KP == 2) {
+                uint32_t w[4];
+                ldsm4t(w, &sm.k[KP - 1][off]);
+                mma_f16(d0, uh[jb], w[0], w[1]);
+                mma_f16(d1, uh[jb], w[2], w[3]);
+            }
+            ldsm4t(b[jb], &sm.k[0][off]);
+            mma_f16(d0, ul[jb], b[jb][0], b[jb][1]);
+            mma_f16(d1, ul[jb], b[jb][2], b[jb][3]);
+        }
+#pragma unroll
+        for (int jb = 0; jb < kNB; jb++) {
+            mma_f16(d0, uh[jb], b[jb][0], b[jb][1]);
+            mma_f16(d1, uh[jb], b[jb][2], b[jb][3]);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            S[2 * nn][c] = fmaf(gamma, S[2 * nn][c], (c < 2 ? iv0 : iv1) * d0[c]);
+            S[2 * nn + 1][c] = fmaf(gamma, S[2 * nn + 1][c], (c < 2 ? iv0 : iv1) * d1[c]);
+        }
+    }
 }
 
 // grid (ceil(rows / 64), hv, requests or segments).
@@ -486,9 +636,8 @@ __device__ __forceinline__ void mma_block(float (&d0)[4], float (&d1)[4], const 
 template <int DK, class T, int kMode>
 __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delta_chunk(ChunkArgs ca) {
     extern __shared__ uint8_t raw[];
-    using Cfg = ChunkCfg<DK, T>;
     constexpr bool kOut = kMode != 1;
-    constexpr int LD = Cfg::LD, KP = Cfg::KP, NT = DK / 8;
+    constexpr int NT = DK / 8;
     ChunkSmem<DK, T>& sm = *reinterpret_cast<ChunkSmem<DK, T>*>(raw);
     const Args& a = ca.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -550,10 +699,11 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
 
     for (uint64_t at = t0; at < t1; at += kC) {
         const int len = (int)min((uint64_t)kC, t1 - at);
-        prepare_chunk<DK, T, kOut>(sm, a, at, len, h, hq, wide);
+        prepare_chunk<DK, T, kOut>(sm, a, at, len, h, hq, wide, warp);
+        __syncthreads();
         if (at + kC < t1) {   // the next chunk's rows on their way to L2
-            const uint64_t r = at + kC + (threadIdx.x >> 1);
-            if (r < t1) {
+            const uint64_t r = at + kC + (threadIdx.x >> 1);   // two threads a row; lanes of the upper half idle
+            if (threadIdx.x < 2 * kC && r < t1) {
                 const char* kn = (const char*)((const T*)a.k + r * a.ld_k + (uint64_t)hq * DK);
                 const char* qn = (const char*)((const T*)a.q + r * a.ld_q + (uint64_t)hq * DK);
 #pragma unroll
@@ -566,179 +716,7 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
                 }
             }
         }
-        if (active) {
-            // X = S K^T and O = S Q^T over the 64 tokens; V meanwhile
-            T V[8][4];
-#pragma unroll
-            for (int n = 0; n < 8; n++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const int i = 8 * n + 2 * t + (c & 1);
-                    V[n][c] = (i < len && !ident) ? vp[(at + i) * a.ld_v + (c >> 1) * 8] : T(0.f);
-                }
-            float X[8][4], O[8][4];
-#pragma unroll
-            for (int n = 0; n < 8; n++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) X[n][c] = O[n][c] = 0.f;
-            float m0 = 0.f, m1 = 0.f;
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                m0 = amax(amax(m0, S[n][0]), S[n][1]);
-                m1 = amax(amax(m1, S[n][2]), S[n][3]);
-            }
-            float sv0, sv1;
-            const float p0 = row_pow(quad_max(m0), sv0), p1 = row_pow(quad_max(m1), sv1);
-            const int brow = (lane & 7) + (lane >> 4) * 8, bcol = ((lane >> 3) & 1) * 8;
-#pragma unroll
-            for (int ks = 0; ks < DK / 16; ks++) {
-                uint32_t hi[4], lo[4];
-                split2(S[2 * ks][0] * p0, S[2 * ks][1] * p0, hi[0], lo[0]);
-                split2(S[2 * ks][2] * p1, S[2 * ks][3] * p1, hi[1], lo[1]);
-                split2(S[2 * ks + 1][0] * p0, S[2 * ks + 1][1] * p0, hi[2], lo[2]);
-                split2(S[2 * ks + 1][2] * p1, S[2 * ks + 1][3] * p1, hi[3], lo[3]);
-#pragma unroll
-                for (int nn = 0; nn < 4; nn++) {
-                    const int off = (nn * 16 + brow) * LD + ks * 16 + bcol;
-                    uint32_t b[4];
-                    if (KP == 2) {
-                        ldsm4(b, &sm.k[KP - 1][off]);
-                        mma_f16(X[2 * nn], hi, b[0], b[1]);
-                        mma_f16(X[2 * nn + 1], hi, b[2], b[3]);
-                    }
-                    ldsm4(b, &sm.k[0][off]);
-                    mma_f16(X[2 * nn], lo, b[0], b[1]);
-                    mma_f16(X[2 * nn + 1], lo, b[2], b[3]);
-                    mma_f16(X[2 * nn], hi, b[0], b[1]);
-                    mma_f16(X[2 * nn + 1], hi, b[2], b[3]);
-                    if (kOut) {
-                        if (KP == 2) {
-                            ldsm4(b, &sm.q[KP - 1][off]);
-                            mma_f16(O[2 * nn], hi, b[0], b[1]);
-                            mma_f16(O[2 * nn + 1], hi, b[2], b[3]);
-                        }
-                        ldsm4(b, &sm.q[0][off]);
-                        mma_f16(O[2 * nn], lo, b[0], b[1]);
-                        mma_f16(O[2 * nn + 1], lo, b[2], b[3]);
-                        mma_f16(O[2 * nn], hi, b[0], b[1]);
-                        mma_f16(O[2 * nn + 1], hi, b[2], b[3]);
-                    }
-                }
-            }
-            // right-hand side b (V - e^c k-norm X), and the state's part of the output
-#pragma unroll
-            for (int n = 0; n < 8; n++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const int i = 8 * n + 2 * t + (c & 1);
-                    const float sv = c < 2 ? sv0 : sv1;
-                    X[n][c] = sm.beta[i] * (to_f32(V[n][c]) - sm.ak[i] * (sv * X[n][c]));
-                    if (kOut) O[n][c] = sm.cq[i] * (sv * O[n][c]);
-                }
-            // solve by blocks of 16 tokens; U takes the place of X
-            uint32_t uh[4][4], ul[4][4];
-            float us[4][2];
-#pragma unroll
-            for (int ib = 0; ib < 4; ib++) {
-                float(&r0)[4] = X[2 * ib];
-                float(&r1)[4] = X[2 * ib + 1];
-                const int i = 16 * ib + 2 * t;
-#pragma unroll
-                for (int jb = 0; jb < ib; jb++) {
-                    float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma_block(d0, d1, uh[jb], ul[jb], sm.m[0], sm.m[1], ib, jb, lane);
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        r0[c] = fmaf(-(sm.ascale[jb][i + (c & 1)] * us[jb][c >> 1]), d0[c], r0[c]);
-                        r1[c] = fmaf(-(sm.ascale[jb][i + 8 + (c & 1)] * us[jb][c >> 1]), d1[c], r1[c]);
-                    }
-                }
-                uint32_t hi[4], lo[4];
-                float inv[2];
-                to_planes(r0, r1, hi, lo, inv);
-                float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_block(d0, d1, hi, lo, sm.m[0], sm.m[1], ib, ib, lane);
-                const float db = sm.dblk[ib];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    r0[c] = d0[c] * (db * inv[c >> 1]);
-                    r1[c] = d1[c] * (db * inv[c >> 1]);
-                }
-                to_planes(r0, r1, uh[ib], ul[ib], us[ib]);
-                if (kOut) {
-#pragma unroll
-                    for (int jb = 0; jb <= ib; jb++) {
-                        float e0[4] = {0.f, 0.f, 0.f, 0.f}, e1[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_block(e0, e1, uh[jb], ul[jb], sm.p[0], sm.p[1], ib, jb, lane);
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            O[2 * ib][c] = fmaf(sm.pscale[jb][i + (c & 1)] * us[jb][c >> 1], e0[c], O[2 * ib][c]);
-                            O[2 * ib + 1][c] = fmaf(sm.pscale[jb][i + 8 + (c & 1)] * us[jb][c >> 1], e1[c], O[2 * ib + 1][c]);
-                        }
-                    }
-                }
-            }
-            if (kOut) {
-#pragma unroll
-                for (int n = 0; n < 8; n++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const int i = 8 * n + 2 * t + (c & 1);
-                        if (i < len) put(op + (at + i) * a.ld_o + (c >> 1) * 8, O[n][c]);
-                    }
-            }
-            // S = e^{c_64} S + sum_j (w_j u_j) k_j^T
-            float n0 = 0.f, n1 = 0.f;
-#pragma unroll
-            for (int n = 0; n < 8; n++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const float w = sm.wk[8 * n + 2 * t + c];
-                    X[n][c] *= w;
-                    X[n][2 + c] *= w;
-                    n0 = amax(n0, X[n][c]);
-                    n1 = amax(n1, X[n][2 + c]);
-                }
-            float iv0, iv1;
-            const float q0 = row_pow(quad_max(n0), iv0), q1 = row_pow(quad_max(n1), iv1);
-#pragma unroll
-            for (int jb = 0; jb < 4; jb++) {
-                split2(X[2 * jb][0] * q0, X[2 * jb][1] * q0, uh[jb][0], ul[jb][0]);
-                split2(X[2 * jb][2] * q1, X[2 * jb][3] * q1, uh[jb][1], ul[jb][1]);
-                split2(X[2 * jb + 1][0] * q0, X[2 * jb + 1][1] * q0, uh[jb][2], ul[jb][2]);
-                split2(X[2 * jb + 1][2] * q1, X[2 * jb + 1][3] * q1, uh[jb][3], ul[jb][3]);
-            }
-            const float gamma = sm.gamma;
-            const int trow = (lane & 7) + ((lane >> 3) & 1) * 8, tcol = (lane >> 4) * 8;
-#pragma unroll
-            for (int nn = 0; nn < NT / 2; nn++) {
-                float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t b[4][4];
-#pragma unroll
-                for (int jb = 0; jb < 4; jb++) {
-                    const int off = (16 * jb + trow) * LD + nn * 16 + tcol;
-                    if (KP == 2) {
-                        uint32_t w[4];
-                        ldsm4t(w, &sm.k[KP - 1][off]);
-                        mma_f16(d0, uh[jb], w[0], w[1]);
-                        mma_f16(d1, uh[jb], w[2], w[3]);
-                    }
-                    ldsm4t(b[jb], &sm.k[0][off]);
-                    mma_f16(d0, ul[jb], b[jb][0], b[jb][1]);
-                    mma_f16(d1, ul[jb], b[jb][2], b[jb][3]);
-                }
-#pragma unroll
-                for (int jb = 0; jb < 4; jb++) {
-                    mma_f16(d0, uh[jb], b[jb][0], b[jb][1]);
-                    mma_f16(d1, uh[jb], b[jb][2], b[jb][3]);
-                }
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    S[2 * nn][c] = fmaf(gamma, S[2 * nn][c], (c < 2 ? iv0 : iv1) * d0[c]);
-                    S[2 * nn + 1][c] = fmaf(gamma, S[2 * nn + 1][c], (c < 2 ? iv0 : iv1) * d1[c]);
-                }
-            }
-        }
+        if (active) consume_chunk<DK, T, kOut>(sm, S, a, vp, op, at, len, ident);
         __syncthreads();   // the shared operands are free again
     }
     if (!active || (kMode == 2 && !last)) return;   // only the last segment's end is the request's
@@ -757,11 +735,27 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
 }
 
 // Start states of a request's segments: S, S M_0 + b_0, ...  grid (ceil(dv / 8), hv, requests), DK threads:
-// thread j owns column j of 8 state rows; bound by the L2 reads of M (DK^2 floats per segment and block).
+// thread j owns column j of 8 state rows.  The chain is one small product per segment; every M and b is
+// there beforehand, so they are copied to shared memory kScanAhead segments early and a step costs its
+// 8 DK^2 products and not the way to L2.
 constexpr int kScanRows = 8;
+__host__ __device__ constexpr int scan_ahead(int dk) { return dk == 128 ? 2 : 4; }
+template <int DK>
+struct alignas(16) ScanSmem {
+    float m[scan_ahead(DK) + 1][DK * DK];
+    float b[scan_ahead(DK) + 1][kScanRows * DK];
+    float4 rows[kScanRows][DK / 4];
+};
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(dst)), "l"(src) : "memory");
+}
+
 template <int DK>
 __global__ void __launch_bounds__(DK) k_delta_scan(ChunkArgs ca) {
-    __shared__ float4 rows[kScanRows][DK / 4];
+    extern __shared__ uint8_t raw[];
+    ScanSmem<DK>& sm = *reinterpret_cast<ScanSmem<DK>*>(raw);
+    constexpr int kAhead = scan_ahead(DK), kBufs = kAhead + 1;
     const Args& a = ca.a;
     const uint32_t h = blockIdx.y, req = blockIdx.z, slot = a.slots[req], j = threadIdx.x, r0 = blockIdx.x * kScanRows;
     const uint64_t t0 = min(a.cu[req], a.n_rows), t1 = min(a.cu[req + 1], a.n_rows), seg = (uint64_t)ca.block * ca.merge;
@@ -777,28 +771,46 @@ __global__ void __launch_bounds__(DK) k_delta_scan(ChunkArgs ca) {
     for (int r = 0; r < kScanRows; r++)
         s[r] = zero ? 0.f : a.state[slot * a.slot_stride + h * per_head + (uint64_t)(r0 + r) * DK + j];
     const uint32_t n_seg = (uint32_t)((t1 - t0 + seg - 1) / seg);
+    const uint64_t first = segment_id(ca, t0, req, 0);
+    const auto fetch = [&](uint32_t p) {   // segment p's M and b, one group of copies (empty past the last)
+        if (p + 1 < n_seg) {
+            const uint64_t id = (first + p) * a.hv + h;
+            const float* m = ca.m_seg + id * (DK * DK);
+            const float* b = ca.b_seg + id * per_head + (uint64_t)r0 * DK;
+            for (int i = j * 4; i < DK * DK; i += DK * 4) copy16(&sm.m[p % kBufs][i], m + i);
+            for (int i = j * 4; i < kScanRows * DK; i += DK * 4) copy16(&sm.b[p % kBufs][i], b + i);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (uint32_t p = 0; p < (uint32_t)kAhead; p++) fetch(p);
     for (uint32_t p = 0; p < n_seg; p++) {
-        const uint64_t id = segment_id(ca, t0, req, p) * a.hv + h;
+        const uint64_t id = (first + p) * a.hv + h;
 #pragma unroll
         for (int r = 0; r < kScanRows; r++) ca.s_in[id * per_head + (uint64_t)(r0 + r) * DK + j] = s[r];
         if (p + 1 == n_seg) break;
+        fetch(p + kAhead);
 #pragma unroll
-        for (int r = 0; r < kScanRows; r++) reinterpret_cast<float*>(rows[r])[j] = s[r];
-        const float* m = ca.m_seg + id * (DK * DK) + j;
-#pragma unroll
-        for (int r = 0; r < kScanRows; r++) s[r] = ca.b_seg[id * per_head + (uint64_t)(r0 + r) * DK + j];
+        for (int r = 0; r < kScanRows; r++) reinterpret_cast<float*>(sm.rows[r])[j] = s[r];
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
         __syncthreads();
-#pragma unroll 8
+        const float* m = sm.m[p % kBufs] + j;
+        float d[kScanRows];
+#pragma unroll
+        for (int r = 0; r < kScanRows; r++) d[r] = 0.f;
+#pragma unroll 4
         for (int k = 0; k < DK / 4; k++) {
             const float m0 = m[(4 * k) * DK], m1 = m[(4 * k + 1) * DK], m2 = m[(4 * k + 2) * DK], m3 = m[(4 * k + 3) * DK];
 #pragma unroll
             for (int r = 0; r < kScanRows; r++) {
-                const float4 x = rows[r][k];
-                s[r] = fmaf(x.x, m0, fmaf(x.y, m1, fmaf(x.z, m2, fmaf(x.w, m3, s[r]))));
+                const float4 x = sm.rows[r][k];
+                d[r] = fmaf(x.x, m0, fmaf(x.y, m1, fmaf(x.z, m2, fmaf(x.w, m3, d[r]))));
             }
         }
-        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kScanRows; r++) s[r] = d[r] + sm.b[p % kBufs][r * DK + j];
+        __syncthreads();   // rows and this buffer are free again
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 }  // namespace delta

@@ -77,6 +77,8 @@ int32_t device(Device** out) {
         d.err = static_cast<uint32_t*>(p);
         OP_CK(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
         OP_CK(cudaFuncSetAttribute(rk::plan::k_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::plan::Smem)));
+        OP_CK(cudaFuncSetAttribute(rk::delta::k_delta_scan<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::delta::ScanSmem<64>)));
+        OP_CK(cudaFuncSetAttribute(rk::delta::k_delta_scan<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::delta::ScanSmem<128>)));
         OP_CK((set_chunk_smem<64, float>()));
         OP_CK((set_chunk_smem<128, float>()));
         OP_CK((set_chunk_smem<64, __nv_bfloat16>()));
@@ -175,7 +177,7 @@ int32_t launch_chunk(const Device& d, rk::delta::ChunkArgs ca, uint32_t max_bloc
         ca.s_in = ca.b_seg + segs * ca.a.hv * ca.a.dv * DK;
         ca.m_seg = ca.s_in + segs * ca.a.hv * ca.a.dv * DK;
         k_delta_chunk<DK, T, 1><<<dim3((unsigned)ceil_div(ca.a.dv + DK, kVRows), ca.a.hv, max_blocks), kCThreads, smem, st>>>(ca);
-        k_delta_scan<DK><<<dim3((unsigned)ceil_div(ca.a.dv, kScanRows), ca.a.hv, ca.a.n), DK, 0, st>>>(ca);
+        k_delta_scan<DK><<<dim3((unsigned)ceil_div(ca.a.dv, kScanRows), ca.a.hv, ca.a.n), DK, sizeof(ScanSmem<DK>), st>>>(ca);
         k_delta_chunk<DK, T, 2><<<dim3(slices, ca.a.hv, max_blocks), kCThreads, smem, st>>>(ca);
     }
     OP_CK(cudaGetLastError());
