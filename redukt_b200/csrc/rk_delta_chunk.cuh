@@ -31,9 +31,7 @@ namespace delta {
 
 constexpr int kC = 32;              // tokens per chunk
 constexpr int kNB = kC / 16;        // 16-token blocks of a chunk
-constexpr int kCWarps = 4;
-constexpr int kCThreads = kCWarps * 32;
-constexpr int kVRows = 16 * kCWarps;  // state rows per block
+constexpr int kPrep = 128;          // threads that prepare a chunk: warps 0-3
 
 // Lower triangle of a kC x kC matrix in two planes, by strips of 16 rows: strip r is 16 (r + 1) wide; a
 // row's stride is an odd number of 16-byte units, so ldmatrix reads 8 rows without a bank conflict.
@@ -42,17 +40,23 @@ constexpr int kStripHalves = 2 * 16 * (24 + 40);
 __host__ __device__ constexpr int strip_ld(int r) { return 16 * r + 24; }
 __host__ __device__ constexpr int strip_base(int r) { return 2 * 16 * (8 * r + 8 * r * (r + 1)); }
 
-template <int DK, class T>
+// Two shapes of a block.  Narrow: 4 warps prepare a chunk, then each steps 16 state rows over it; several blocks
+// share an SM and fill one another's waits.  Wide: 4 warps prepare the next chunk while 8 others step 128
+// state rows over the present one, so a 128-row head prepares its chunks once instead of twice.
+template <int DK, class T, bool kWide>
 struct ChunkCfg {
     static constexpr bool kF32 = sizeof(T) == 4;
     static constexpr int KP = kF32 ? 2 : 1;     // planes of k and q
     static constexpr int LD = DK + 8;           // halves per row of a plane
-    static constexpr int kMinBlocks = DK == 64 ? 4 : 3;
+    static constexpr int kThreads = kWide ? 384 : 128;
+    static constexpr int kRows = kWide ? 128 : 64;   // state rows per block
+    static constexpr int kMinBlocks = kWide ? 1 : DK == 64 ? 4 : kF32 ? 2 : 3;   // what registers and shared memory allow
 };
 
+// A prepared chunk.
 template <int DK, class T>
-struct alignas(16) ChunkSmem {
-    using Cfg = ChunkCfg<DK, T>;
+struct alignas(16) Chunk {
+    using Cfg = ChunkCfg<DK, T, false>;
     __half k[Cfg::KP][kC * Cfg::LD];
     __half q[Cfg::KP][kC * Cfg::LD];
     __half m[kStripHalves];             // B below the diagonal blocks, D on them; before that, A in f32
@@ -65,6 +69,12 @@ struct alignas(16) ChunkSmem {
     float rf[16], cf[16];               // block (1, 0): e^{c_i - c_15} of its rows, e^{c_15 - c_j} of its columns
     float pscale[kNB][kC];              // scale of a row of each 16 x 16 block of P
     float dscale[kNB], bscale;          // scales of D and B
+};
+
+template <int DK, class T, bool kWide>
+struct alignas(16) ChunkSmem {
+    Chunk<DK, T> c[kWide ? 2 : 1];
+    uint4 raw[kPrep * 4 * (DK * (int)sizeof(T) / 128)];   // the next chunk's k and q, each thread's own vectors
 };
 
 struct ChunkArgs {
@@ -126,7 +136,9 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const __half* p) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(tc::smem_u32(p)) : "memory");
 }
 
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(dst)), "l"(src) : "memory");
+}
 
 // One row of DK values of type T to f16 planes: 8 lanes a row, lane l of the eight takes the 16-byte
 // vectors l, l + 8, ...
@@ -134,15 +146,24 @@ template <int DK, class T>
 struct RowLoad {
     static constexpr int N = 16 / sizeof(T), NV = DK / N / 8;
     uint4 raw[NV];
-    __device__ __forceinline__ void load(const T* p, int l) {
+    // Vectors of a row on their way to this thread's slots of the staging area, and back from there.
+    static __device__ __forceinline__ void stage(uint4* slot, const T* p, bool wide, int l) {
 #pragma unroll
-        for (int i = 0; i < NV; i++) raw[i] = *reinterpret_cast<const uint4*>(p + (l + 8 * i) * N);
+        for (int i = 0; i < NV; i++) {
+            const T* v = p + (l + 8 * i) * N;
+            if (wide) {
+                copy16(slot + i * kPrep, v);
+            } else {   // any alignment
+                uint4 w;
+#pragma unroll
+                for (int c = 0; c < N; c++) reinterpret_cast<T*>(&w)[c] = v[c];
+                slot[i * kPrep] = w;
+            }
+        }
     }
-    __device__ __forceinline__ void load_single(const T* p, int l) {   // any alignment
+    __device__ __forceinline__ void unstage(const uint4* slot) {
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-#pragma unroll
-            for (int c = 0; c < N; c++) reinterpret_cast<T*>(&raw[i])[c] = p[(l + 8 * i) * N + c];
+        for (int i = 0; i < NV; i++) raw[i] = slot[i * kPrep];
     }
     __device__ __forceinline__ void clear_unless(bool live) {
 #pragma unroll
@@ -213,39 +234,65 @@ __device__ __forceinline__ void put_rows(RowLoad<DK, T> (&x)[4], __half* hi, __h
 }
 
 // A barrier of the four warps that prepare a chunk.
-__device__ __forceinline__ void prep_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kCThreads) : "memory"); }
+__device__ __forceinline__ void prep_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPrep) : "memory"); }
 
 // Where A's value (row of the strip, column) waits for the substitution: by columns of 16 floats, their
 // four 16-byte parts swapped so that the mma layout's stores meet two to a bank at most.
 __device__ __forceinline__ int wait_at(int row, int col) { return col * 16 + ((((row >> 2) ^ (col >> 1)) & 3) << 2) + (row & 3); }
 
-// Fills the chunk's shared operands: planes and scales of k and q, decay factors, D and B, and P.  Run by
-// four warps (`warp` 0..3); the caller's barrier publishes the last writes.
+// What the four preparing warps bring from one chunk to the next.
 template <int DK, class T, bool kOut>
-__device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& a, uint64_t t0, int len, uint32_t h, uint32_t hq,
-                                              bool wide, int warp) {
-    using Cfg = ChunkCfg<DK, T>;
-    constexpr int LD = Cfg::LD, KP = Cfg::KP;
-    const int lane = threadIdx.x & 31, grp = lane >> 3, l = lane & 7, g = lane >> 2, t = lane & 3;
-    const bool key = warp < 2;                    // warps 0 and 1 bring k's rows, 2 and 3 q's
-    const int row = (warp & 1) * 16 + grp;
-    RowLoad<DK, T> rows[4];
-    if (kOut || key) {
-        const T* p = key ? (const T*)a.k + t0 * a.ld_k + (uint64_t)hq * DK : (const T*)a.q + t0 * a.ld_q + (uint64_t)hq * DK;
-        const uint64_t ld = key ? a.ld_k : a.ld_q;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {   // rows past the end read the last one and are cleared
-            const uint32_t r = min(row + 4 * i, len - 1);
-            if (wide) rows[i].load(p + r * ld, l);
-            else rows[i].load_single(p + r * ld, l);
-        }
+struct Source {
+    const T* p;             // this thread's first row: k's for warps 0 and 1, q's for 2 and 3
+    uint64_t ld;
+    const float *g, *beta;  // of token `lane`
+    uint64_t ld_g;
+    float gate, b;          // the staged chunk's
+    int warp, row, l;       // row of the 8-lane group in the chunk, lane in it
+    bool wide;
+
+    __device__ __forceinline__ void init(const Args& a, uint64_t t0, uint32_t h, uint32_t hq) {
+        const int lane = threadIdx.x & 31;
+        warp = threadIdx.x >> 5;
+        row = (warp & 1) * 16 + (lane >> 3);
+        l = lane & 7;
+        ld = warp < 2 ? a.ld_k : a.ld_q;
+        p = (const T*)(warp < 2 ? a.k : a.q) + (t0 + row) * ld + (uint64_t)hq * DK;
+        wide = ((reinterpret_cast<uintptr_t>(warp < 2 ? a.k : a.q) | (ld * sizeof(T))) & 15) == 0;
+        g = a.g + (t0 + lane) * a.ld_g + h;
+        beta = a.beta + (t0 + lane) * a.ld_g + h;
+        ld_g = a.ld_g;
     }
-    if (warp != 1) {   // the warps have c of token `lane`; each writes its share of the factors
-        double s = 0.0;
-        if (lane < len) {
-            const float x = a.g[(t0 + lane) * a.ld_g + h];
-            s = x < -1000.f ? -1000.0 : (double)x;   // e^-1000 is 0 in f32; -inf - -inf would be NaN
+    // Starts the copies of the next chunk of `len` tokens; rows past its end repeat the last one.
+    __device__ __forceinline__ void stage(uint4* raw, int len) {
+        if (kOut || warp < 2) {
+            uint4* slot = raw + threadIdx.x;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = min(row + 4 * i, len - 1) - row;
+                RowLoad<DK, T>::stage(slot + i * RowLoad<DK, T>::NV * kPrep, p + (int64_t)r * (int64_t)ld, wide, l);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            p += kC * ld;
         }
+        const bool live = (int)(threadIdx.x & 31) < len;
+        gate = live && warp != 1 ? *g : 0.f;
+        b = live && warp == 1 ? *beta : 0.f;
+        g += kC * ld_g;
+        beta += kC * ld_g;
+    }
+};
+
+// Fills the chunk's shared operands from the staged rows: planes and scales of k and q, decay factors, D
+// and B, and P.  Run by four warps; the caller's barrier publishes the last writes.
+template <int DK, class T, bool kOut>
+__device__ __forceinline__ void prepare_chunk(Chunk<DK, T>& sm, const uint4* raw, const Args& a, const Source<DK, T, kOut>& src, int len) {
+    using Cfg = ChunkCfg<DK, T, false>;
+    constexpr int LD = Cfg::LD, KP = Cfg::KP;
+    const int lane = threadIdx.x & 31, l = src.l, g = lane >> 2, t = lane & 3, warp = src.warp, row = src.row;
+    const bool key = warp < 2;
+    if (warp != 1) {   // the warps have c of token `lane`; each writes its share of the factors
+        double s = src.gate < -1000.f ? -1000.0 : (double)src.gate;   // e^-1000 is 0 in f32; -inf - -inf would be NaN
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double y = __shfl_up_sync(0xFFFFFFFFu, s, o);
@@ -266,18 +313,23 @@ __device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& 
             (lane < 16 ? sm.cf : sm.rf)[lane & 15] = x;
         }
     } else {
-        sm.beta[lane] = lane < len ? a.beta[(t0 + lane) * a.ld_g + h] : 0.f;
+        sm.beta[lane] = src.b;
     }
-    if (kOut || key)
+    if (kOut || key) {
+        RowLoad<DK, T> rows[4];
+        asm volatile("cp.async.wait_all;" ::: "memory");   // this thread's own copies
+#pragma unroll
+        for (int i = 0; i < 4; i++) rows[i].unstage(raw + threadIdx.x + i * RowLoad<DK, T>::NV * kPrep);
         put_rows<DK, T>(rows, key ? sm.k[0] : sm.q[0], key ? sm.k[KP - 1] : sm.q[KP - 1], LD, key ? sm.sk : sm.sq, row, len, a.l2norm, l);
+    }
     prep_sync();
     if (warp == 3) {
         sm.ak[lane] = sm.ee[lane] * sm.sk[lane];
         sm.wk[lane] *= sm.sk[lane];
         if (kOut) sm.cq[lane] = a.scale * sm.ee[lane] * sm.sq[lane];
     }
-    // Strip r of a product is rows 16 r .. 16 r + 15 against tokens 0 .. 16 r + 15, slot s of it the tokens 16 s ..
-    // Warps 0 and 2 do strips 1 and 0 of K K^T, warps 1 and 3 those of Q K^T.
+    // Strip r of a product is rows 16 r .. 16 r + 15 against tokens 0 .. 16 r + 15: slot 0 its diagonal block, slot 1
+    // the block beside it (strip 1).  Warps 0 and 2 do strips 1 and 0 of K K^T, warps 1 and 3 those of Q K^T.
     const bool gram = (warp & 1) == 0;
     const int r = 1 - (warp >> 1);
     if (!kOut && !gram) return;
@@ -299,11 +351,12 @@ __device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& 
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 if (s > r) continue;
+                const int off = (s ? 0 : r * 16 * LD) + boff + ks * 16;
                 uint32_t fb[4];
-                ldsm4(fb, &sm.k[0][s * 16 * LD + boff + ks * 16]);
+                ldsm4(fb, &sm.k[0][off]);
                 if (KP == 2) {
                     uint32_t fw[4];
-                    ldsm4(fw, &sm.k[KP - 1][s * 16 * LD + boff + ks * 16]);
+                    ldsm4(fw, &sm.k[KP - 1][off]);
                     mma_f16(acc[s][0], fa, fw[0], fw[1]);
                     mma_f16(acc[s][1], fa, fw[2], fw[3]);
                     mma_f16(acc[s][0], fl, fb[0], fb[1]);
@@ -323,18 +376,18 @@ __device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& 
     const float k1 = gram ? sm.beta[i0 + 8] * sm.sk[i0 + 8] : a.scale * sm.sq[i0 + 8];
     const float ch0 = sm.chi[i0], cl0 = sm.clo[i0], ch1 = sm.chi[i0 + 8], cl1 = sm.clo[i0 + 8];
 #pragma unroll
-    for (int s = 0; s < 2; s++) {   // columns 16 s + 8 n + 2 t + c; s == r is the diagonal block
+    for (int s = 0; s < 2; s++) {
         if (s > r) continue;
-        const bool diag = s == r;
+        const int nb = s ? 0 : r;   // columns 16 nb + 8 n + 2 t + c
         const float f0 = k0 * sm.rf[g], f1 = k1 * sm.rf[g + 8];
         float m0 = 0.f, m1 = 0.f;
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                const int jj = 8 * n + 2 * t + c, j = 16 * s + jj;
+                const int jj = 8 * n + 2 * t + c, j = 16 * nb + jj;
                 const float kj = sm.sk[j];
-                if (diag) {   // every pair's own exponent
+                if (s == 0) {   // every pair's own exponent
                     const float hj = sm.chi[j], lj = sm.clo[j];
                     const float e0 = exp2f((ch0 - hj) + (cl0 - lj)), e1 = exp2f((ch1 - hj) + (cl1 - lj));
                     acc[s][n][c] = jj < g + !gram ? acc[s][n][c] * (k0 * kj) * e0 : 0.f;
@@ -355,12 +408,12 @@ __device__ __forceinline__ void prepare_chunk(ChunkSmem<DK, T>& sm, const Args& 
         float v0, v1;
         const float p0 = row_pow(quad_max(m0), v0), p1 = row_pow(quad_max(m1), v1);
         if (t == 0) {
-            sm.pscale[s][i0] = v0;
-            sm.pscale[s][i0 + 8] = v1;
+            sm.pscale[nb][i0] = v0;
+            sm.pscale[nb][i0 + 8] = v1;
         }
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-            const int at = g * ld + 16 * s + 8 * n + 2 * t;
+            const int at = g * ld + 16 * nb + 8 * n + 2 * t;
             uint32_t x, y;
             split2(acc[s][n][0] * p0, acc[s][n][1] * p0, x, y);
             *reinterpret_cast<uint32_t*>(hi + at) = x;
@@ -448,9 +501,9 @@ __device__ __forceinline__ void mma_block(float (&d0)[4], float (&d1)[4], const 
 // One chunk's step of 16 state rows, by one warp: S (rows row0 + g and + 8, columns 8 n + 2 t, + 1) to the
 // state after it, with outputs where kOut.  vp and op: v and out at (row 0, this thread's first state row).
 template <int DK, class T, bool kOut>
-__device__ __forceinline__ void consume_chunk(const ChunkSmem<DK, T>& sm, float (&S)[DK / 8][4], const Args& a, const T* vp, T* op,
+__device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)[DK / 8][4], const Args& a, const T* vp, T* op,
                                               uint64_t at, int len, bool ident) {
-    using Cfg = ChunkCfg<DK, T>;
+    using Cfg = ChunkCfg<DK, T, false>;
     constexpr int LD = Cfg::LD, KP = Cfg::KP, NT = DK / 8;
     const int lane = threadIdx.x & 31, t = lane & 3;
     // X = S K^T and O = S Q^T over the chunk; V meanwhile
@@ -628,17 +681,18 @@ __device__ __forceinline__ void consume_chunk(const ChunkSmem<DK, T>& sm, float 
     }
 }
 
-// grid (ceil(rows / 64), hv, requests or segments).
+// grid (ceil(rows / kRows), hv, requests or segments).
 // kMode 0: whole requests, state from and to the slots.
 // kMode 1: a segment's transition: rows below dv from zero state, rows dv .. dv + DK the identity with
 //          v = 0; end states to b_seg and m_seg, no outputs.
 // kMode 2: a segment from its start state in s_in, with outputs; the request's last one writes the slot.
-template <int DK, class T, int kMode>
-__global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delta_chunk(ChunkArgs ca) {
+template <int DK, class T, bool kWide, int kMode>
+__global__ void __launch_bounds__(ChunkCfg<DK, T, kWide>::kThreads, ChunkCfg<DK, T, kWide>::kMinBlocks) k_delta_chunk(ChunkArgs ca) {
     extern __shared__ uint8_t raw[];
+    using Cfg = ChunkCfg<DK, T, kWide>;
     constexpr bool kOut = kMode != 1;
     constexpr int NT = DK / 8;
-    ChunkSmem<DK, T>& sm = *reinterpret_cast<ChunkSmem<DK, T>*>(raw);
+    ChunkSmem<DK, T, kWide>& sm = *reinterpret_cast<ChunkSmem<DK, T, kWide>*>(raw);
     const Args& a = ca.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t h = blockIdx.y, hq = h / (a.hv / a.hk);
@@ -660,24 +714,22 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
         t1 = min(t1, t0 + seg);
         if (kMode == 1 && last) return;               // nothing starts from its end
     }
-    const int row0 = blockIdx.x * kVRows + warp * 16;  // this warp's first state row
+    const int row0 = blockIdx.x * Cfg::kRows + (kWide ? warp - 4 : warp) * 16;  // this warp's first state row
     if (slot >= a.n_slots) {   // only this request is rejected: zero outputs, no state touched
         if (kOut) {
-            const uint32_t r0 = blockIdx.x * kVRows, w = min(a.dv, r0 + kVRows) - r0;
-            for (uint64_t i = threadIdx.x; i < (t1 - t0) * w; i += kCThreads)
+            const uint32_t r0 = blockIdx.x * Cfg::kRows, w = min(a.dv, r0 + Cfg::kRows) - r0;
+            for (uint64_t i = threadIdx.x; i < (t1 - t0) * w; i += Cfg::kThreads)
                 put((T*)a.out + (t0 + i / w) * a.ld_o + (uint64_t)h * a.dv + r0 + i % w, 0.f);
             if (t1 > t0 && h == 0 && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err, 1u);
         }
         return;
     }
     const bool ident = kMode == 1 && row0 >= (int)a.dv;
-    const bool active = row0 < (int)a.dv + (kMode == 1 ? DK : 0);
+    const bool active = row0 < (int)a.dv + (kMode == 1 ? DK : 0) && (!kWide || warp >= 4);
     const uint64_t per_head = (uint64_t)a.dv * DK;
     float* st = a.state + slot * a.slot_stride + h * per_head;
     const float* src = kMode == 2 ? ca.s_in + seg_head * per_head : st;
     const bool zero = kMode == 1 || (kMode == 0 && a.fresh && a.fresh[req]);
-    const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | (a.ld_q * sizeof(T)) | (a.ld_k * sizeof(T))) & 15) == 0;
-
     float S[NT][4];   // rows row0 + g and + 8, columns 8 n + 2 t, + 1
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -697,27 +749,34 @@ __global__ void __launch_bounds__(kCThreads, ChunkCfg<DK, T>::kMinBlocks) k_delt
     const T* vp = (const T*)a.v + (uint64_t)h * a.dv + row0 + g;
     T* op = (T*)a.out + (uint64_t)h * a.dv + row0 + g;
 
-    for (uint64_t at = t0; at < t1; at += kC) {
-        const int len = (int)min((uint64_t)kC, t1 - at);
-        prepare_chunk<DK, T, kOut>(sm, a, at, len, h, hq, wide, warp);
-        __syncthreads();
-        if (at + kC < t1) {   // the next chunk's rows on their way to L2
-            const uint64_t r = at + kC + (threadIdx.x >> 1);   // two threads a row; lanes of the upper half idle
-            if (threadIdx.x < 2 * kC && r < t1) {
-                const char* kn = (const char*)((const T*)a.k + r * a.ld_k + (uint64_t)hq * DK);
-                const char* qn = (const char*)((const T*)a.q + r * a.ld_q + (uint64_t)hq * DK);
-#pragma unroll
-                for (int b = 0; b < DK * (int)sizeof(T); b += 256) {
-                    const int o = b + (threadIdx.x & 1) * 128;
-                    if (o < DK * (int)sizeof(T)) {
-                        prefetch_l2(kn + o);
-                        if (kOut) prefetch_l2(qn + o);
-                    }
-                }
+    const auto chunk_len = [&](uint64_t at) { return (int)min((uint64_t)kC, t1 - at); };
+    if constexpr (kWide) {
+        if (warp < 4) {
+            Source<DK, T, kOut> in;
+            in.init(a, t0, h, hq);
+            if (t0 < t1) in.stage(sm.raw, chunk_len(t0));
+            for (uint64_t at = t0, n = 0; at < t1; at += kC, n++) {
+                prepare_chunk<DK, T, kOut>(sm.c[n & 1], sm.raw, a, in, chunk_len(at));
+                if (at + kC < t1) in.stage(sm.raw, chunk_len(at + kC));
+                __syncthreads();   // chunk n is there, and chunk n - 1's buffer free
             }
+            return;
         }
-        if (active) consume_chunk<DK, T, kOut>(sm, S, a, vp, op, at, len, ident);
-        __syncthreads();   // the shared operands are free again
+        for (uint64_t at = t0, n = 0; at < t1; at += kC, n++) {
+            __syncthreads();
+            if (active) consume_chunk<DK, T, kOut>(sm.c[n & 1], S, a, vp, op, at, chunk_len(at), ident);
+        }
+    } else {
+        Source<DK, T, kOut> in;
+        in.init(a, t0, h, hq);
+        if (t0 < t1) in.stage(sm.raw, chunk_len(t0));
+        for (uint64_t at = t0; at < t1; at += kC) {
+            prepare_chunk<DK, T, kOut>(sm.c[0], sm.raw, a, in, chunk_len(at));
+            if (at + kC < t1) in.stage(sm.raw, chunk_len(at + kC));
+            __syncthreads();
+            if (active) consume_chunk<DK, T, kOut>(sm.c[0], S, a, vp, op, at, chunk_len(at), ident);
+            __syncthreads();   // the shared operands are free again
+        }
     }
     if (!active || (kMode == 2 && !last)) return;   // only the last segment's end is the request's
     float* dst = st;
@@ -746,10 +805,6 @@ struct alignas(16) ScanSmem {
     float b[scan_ahead(DK) + 1][kScanRows * DK];
     float4 rows[kScanRows][DK / 4];
 };
-
-__device__ __forceinline__ void copy16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(dst)), "l"(src) : "memory");
-}
 
 template <int DK>
 __global__ void __launch_bounds__(DK) k_delta_scan(ChunkArgs ca) {

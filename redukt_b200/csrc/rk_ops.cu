@@ -55,12 +55,13 @@ cudaError_t set_smem() {
     return cudaFuncSetAttribute(rk::w8::k_w8a8_tc<BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rk::w8::tc_smem<BN>());
 }
 
-template <int DK, class T>
+template <int DK, class T, bool kWide>
 cudaError_t set_chunk_smem() {
-    const int bytes = (int)sizeof(rk::delta::ChunkSmem<DK, T>);
-    if (cudaError_t e = cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
-    if (cudaError_t e = cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
-    return cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const int bytes = (int)sizeof(rk::delta::ChunkSmem<DK, T, kWide>);
+    const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    if (cudaError_t e = cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, kWide, 0>, attr, bytes)) return e;
+    if (cudaError_t e = cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, kWide, 1>, attr, bytes)) return e;
+    return cudaFuncSetAttribute(rk::delta::k_delta_chunk<DK, T, kWide, 2>, attr, bytes);
 }
 
 // The current device's facts; the first call on a device looks them up and sets the kernels'
@@ -79,10 +80,12 @@ int32_t device(Device** out) {
         OP_CK(cudaFuncSetAttribute(rk::plan::k_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::plan::Smem)));
         OP_CK(cudaFuncSetAttribute(rk::delta::k_delta_scan<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::delta::ScanSmem<64>)));
         OP_CK(cudaFuncSetAttribute(rk::delta::k_delta_scan<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::delta::ScanSmem<128>)));
-        OP_CK((set_chunk_smem<64, float>()));
-        OP_CK((set_chunk_smem<128, float>()));
-        OP_CK((set_chunk_smem<64, __nv_bfloat16>()));
-        OP_CK((set_chunk_smem<128, __nv_bfloat16>()));
+        OP_CK((set_chunk_smem<64, float, false>()));
+        OP_CK((set_chunk_smem<64, __nv_bfloat16, false>()));
+        OP_CK((set_chunk_smem<128, float, false>()));
+        OP_CK((set_chunk_smem<128, __nv_bfloat16, false>()));
+        OP_CK((set_chunk_smem<128, float, true>()));
+        OP_CK((set_chunk_smem<128, __nv_bfloat16, true>()));
         OP_CK((set_smem<256, float>()));
         OP_CK((set_smem<256, __nv_bfloat16>()));
         OP_CK((set_smem<128, float>()));
@@ -143,45 +146,55 @@ uint64_t seg_floats(uint64_t hv, uint64_t dk, uint64_t dv) { return hv * dk * (2
 // Table blocks per segment, 0 = the requests are not cut.  Estimated time in chunk steps of one block alone
 // on its SM: co-resident blocks slow one another by about 0.4 of a step each, blocks past the
 // resident ones wait for a wave.  The transition pass has the key's rows beside the value's and, with
-// no outputs, steps of about 0.7; a scan step is about 0.1.  Only the requests' mean length is
+// no outputs, steps of about 0.7; a scan step is about 0.5.  Only the requests' mean length is
 // known here.  16,384 tokens of one request, 8 heads of 128: 2.71 ms uncut.
-uint32_t segment_merge(const Device& d, const rk::delta::Args& a, uint32_t dk, uint32_t block, int resident, uint64_t work_bytes) {
+uint32_t segment_merge(const Device& d, const rk::delta::Args& a, uint32_t dk, uint32_t block, int rows, int resident, uint64_t work_bytes) {
     const auto steps = [&](double blocks) {
         const double k = blocks / d.sms, waves = std::ceil(blocks / (double)(d.sms * resident));
         return waves * (1.0 + 0.4 * (std::max(1.0, std::min(k, (double)resident)) - 1.0));
     };
-    const double slices = (double)ceil_div(a.dv, rk::delta::kVRows), both = (double)ceil_div(a.dv + dk, rk::delta::kVRows);
+    const double slices = (double)ceil_div(a.dv, rows), both = (double)ceil_div(a.dv + dk, rows);
     double best = 0.8 * (double)a.n_rows / rk::delta::kC / a.n * steps(a.n * (double)a.hv * slices);
     uint32_t merge = 0;
     for (uint32_t m = 1; (uint64_t)m * block * a.n <= a.n_rows; m *= 2) {
         const uint64_t segs = a.n_rows / ((uint64_t)m * block) + a.n;
         if (segs * seg_floats(a.hv, dk, a.dv) * 4 > work_bytes) continue;
         const double chunks = (double)m * block / rk::delta::kC;
-        const double t = chunks * (0.7 * steps(segs * (double)a.hv * both) + steps(segs * (double)a.hv * slices)) + 0.1 * segs / a.n + 1.0;
+        const double t = chunks * (0.7 * steps(segs * (double)a.hv * both) + steps(segs * (double)a.hv * slices)) + 0.5 * segs / a.n + 1.0;
         if (t < best) best = t, merge = m;
     }
     return merge;
 }
 
-template <int DK, class T>
+template <int DK, class T, bool kWide>
 int32_t launch_chunk(const Device& d, rk::delta::ChunkArgs ca, uint32_t max_blocks, void* d_work, uint64_t work_bytes, cudaStream_t st) {
     using namespace rk::delta;
-    const unsigned slices = (unsigned)ceil_div(ca.a.dv, kVRows), smem = (unsigned)sizeof(ChunkSmem<DK, T>);
-    if (ca.blocks && d_work) ca.merge = segment_merge(d, ca.a, DK, ca.block, ChunkCfg<DK, T>::kMinBlocks, work_bytes);
+    using Cfg = ChunkCfg<DK, T, kWide>;
+    const unsigned slices = (unsigned)ceil_div(ca.a.dv, Cfg::kRows), smem = (unsigned)sizeof(ChunkSmem<DK, T, kWide>);
+    if (ca.blocks && d_work) ca.merge = segment_merge(d, ca.a, DK, ca.block, Cfg::kRows, Cfg::kMinBlocks, work_bytes);
     else ca.merge = 0;
     if (!ca.merge) {
-        k_delta_chunk<DK, T, 0><<<dim3(slices, ca.a.hv, ca.a.n), kCThreads, smem, st>>>(ca);
+        k_delta_chunk<DK, T, kWide, 0><<<dim3(slices, ca.a.hv, ca.a.n), Cfg::kThreads, smem, st>>>(ca);
     } else {
         const uint64_t segs = ca.a.n_rows / ((uint64_t)ca.merge * ca.block) + ca.a.n;
         ca.b_seg = static_cast<float*>(d_work);
         ca.s_in = ca.b_seg + segs * ca.a.hv * ca.a.dv * DK;
         ca.m_seg = ca.s_in + segs * ca.a.hv * ca.a.dv * DK;
-        k_delta_chunk<DK, T, 1><<<dim3((unsigned)ceil_div(ca.a.dv + DK, kVRows), ca.a.hv, max_blocks), kCThreads, smem, st>>>(ca);
+        k_delta_chunk<DK, T, kWide, 1><<<dim3((unsigned)ceil_div(ca.a.dv + DK, Cfg::kRows), ca.a.hv, max_blocks), Cfg::kThreads, smem, st>>>(ca);
         k_delta_scan<DK><<<dim3((unsigned)ceil_div(ca.a.dv, kScanRows), ca.a.hv, ca.a.n), DK, sizeof(ScanSmem<DK>), st>>>(ca);
-        k_delta_chunk<DK, T, 2><<<dim3(slices, ca.a.hv, max_blocks), kCThreads, smem, st>>>(ca);
+        k_delta_chunk<DK, T, kWide, 2><<<dim3(slices, ca.a.hv, max_blocks), Cfg::kThreads, smem, st>>>(ca);
     }
     OP_CK(cudaGetLastError());
     return BACKEND_OK;
+}
+
+// 128 value rows per block where there are that many to fill it, 64 otherwise.
+template <class T>
+int32_t launch_chunk_t(const Device& d, const rk::delta::ChunkArgs& ca, uint32_t dk, uint32_t max_blocks, void* d_work, uint64_t work_bytes,
+                       cudaStream_t st) {
+    if (dk == 64) return launch_chunk<64, T, false>(d, ca, max_blocks, d_work, work_bytes, st);
+    if (ca.a.dv <= 64) return launch_chunk<128, T, false>(d, ca, max_blocks, d_work, work_bytes, st);
+    return launch_chunk<128, T, true>(d, ca, max_blocks, d_work, work_bytes, st);
 }
 
 // ---- 8-bit product ----
@@ -372,11 +385,8 @@ int32_t redukt_b200_delta_chunk(const void* d_q, const void* d_k, const void* d_
     a.cu = d_cu;
     const cudaStream_t st = stream_of(cuda_stream);
     rk::delta::ChunkArgs ca = {a, d_blocks, block, 0, nullptr, nullptr, nullptr};
-    if (dtype == REDUKT_DTYPE_F32)
-        return d_key == 64 ? launch_chunk<64, float>(*d, ca, max_blocks, d_work, work_bytes, st)
-                           : launch_chunk<128, float>(*d, ca, max_blocks, d_work, work_bytes, st);
-    return d_key == 64 ? launch_chunk<64, __nv_bfloat16>(*d, ca, max_blocks, d_work, work_bytes, st)
-                       : launch_chunk<128, __nv_bfloat16>(*d, ca, max_blocks, d_work, work_bytes, st);
+    return dtype == REDUKT_DTYPE_F32 ? launch_chunk_t<float>(*d, ca, d_key, max_blocks, d_work, work_bytes, st)
+                                     : launch_chunk_t<__nv_bfloat16>(*d, ca, d_key, max_blocks, d_work, work_bytes, st);
 }
 
 int32_t redukt_b200_quantize_tokens(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q,
