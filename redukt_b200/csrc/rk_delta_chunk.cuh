@@ -123,9 +123,9 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const __half* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -205,6 +205,12 @@ struct RowLoad {
     }
 };
 
+// 1 / sqrt(x): the hardware's estimate and one Newton step.
+__device__ __forceinline__ float inv_sqrt(float x) {
+    const float y = rsqrtf(x);
+    return y * fmaf(-0.5f * x * y, y, 1.5f);
+}
+
 // Four rows of each 8-lane group: row, row + 4, row + 8, row + 12.
 template <int DK, class T>
 __device__ __forceinline__ void put_rows(RowLoad<DK, T> (&x)[4], __half* hi, __half* lo, int ld, float* scale, int row, int len, bool l2norm, int l) {
@@ -227,7 +233,7 @@ __device__ __forceinline__ void put_rows(RowLoad<DK, T> (&x)[4], __half* hi, __h
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         s[i] = row_pow(m[i], inv[i]);
-        if (l2norm) inv[i] *= 1.f / sqrtf(ss[i] + kNormEps);
+        if (l2norm) inv[i] *= inv_sqrt(ss[i] + kNormEps);
         x[i].put(hi + (row + 4 * i) * ld, lo + (row + 4 * i) * ld, s[i], l);
         if (l == 0) scale[row + 4 * i] = inv[i];
     }
@@ -240,18 +246,22 @@ __device__ __forceinline__ void prep_sync() { asm volatile("bar.sync 1, %0;" ::"
 // four 16-byte parts swapped so that the mma layout's stores meet two to a bank at most.
 __device__ __forceinline__ int wait_at(int row, int col) { return col * 16 + ((((row >> 2) ^ (col >> 1)) & 3) << 2) + (row & 3); }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // What the four preparing warps bring from one chunk to the next.
 template <int DK, class T, bool kOut>
 struct Source {
     const T* p;             // this thread's first row: k's for warps 0 and 1, q's for 2 and 3
     uint64_t ld;
     const float *g, *beta;  // of token `lane`
-    uint64_t ld_g;
+    const T* v;             // token threadIdx.x / 4 of the chunk: the block's value rows
+    uint64_t ld_g, ld_v;
     float gate, b;          // the staged chunk's
     int warp, row, l;       // row of the 8-lane group in the chunk, lane in it
     bool wide;
+    uint32_t v_bytes;
 
-    __device__ __forceinline__ void init(const Args& a, uint64_t t0, uint32_t h, uint32_t hq) {
+    __device__ __forceinline__ void init(const Args& a, uint64_t t0, uint32_t h, uint32_t hq, uint32_t v_row, uint32_t v_rows) {
         const int lane = threadIdx.x & 31;
         warp = threadIdx.x >> 5;
         row = (warp & 1) * 16 + (lane >> 3);
@@ -262,6 +272,9 @@ struct Source {
         g = a.g + (t0 + lane) * a.ld_g + h;
         beta = a.beta + (t0 + lane) * a.ld_g + h;
         ld_g = a.ld_g;
+        ld_v = a.ld_v;
+        v = (const T*)a.v + (t0 + (threadIdx.x >> 2)) * ld_v + (uint64_t)h * a.dv + v_row;
+        v_bytes = v_row < a.dv ? min(v_rows, a.dv - v_row) * (uint32_t)sizeof(T) : 0u;
     }
     // Starts the copies of the next chunk of `len` tokens; rows past its end repeat the last one.
     __device__ __forceinline__ void stage(uint4* raw, int len) {
@@ -280,6 +293,9 @@ struct Source {
         b = live && warp == 1 ? *beta : 0.f;
         g += kC * ld_g;
         beta += kC * ld_g;
+        if ((int)(threadIdx.x >> 2) < len)   // the values, read straight from global memory, on their way to L2
+            for (uint32_t o = (threadIdx.x & 3) * 128; o < v_bytes; o += 512) prefetch_l2((const char*)v + o);
+        v += kC * ld_v;
     }
 };
 
@@ -484,19 +500,23 @@ __device__ __forceinline__ void to_planes(const float (&x)[4], const float (&y)[
 }
 
 // d0, d1 (16 columns) += planes x a 16 x 16 block of a strip matrix (rows i = columns of the result)
-__device__ __forceinline__ void mma_block(float (&d0)[4], float (&d1)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4],
-                                          const __half* strips, int ib, int jb, int lane) {
-    const __half* at = strips + strip_base(ib) + ((lane & 7) + (lane >> 4) * 8) * strip_ld(ib) + 16 * jb + ((lane >> 3) & 1) * 8;
-    uint32_t b[4], w[4];
-    ldsm4(w, at + 16 * strip_ld(ib));
-    ldsm4(b, at);
-    mma_f16(d0, hi, w[0], w[1]);
-    mma_f16(d1, hi, w[2], w[3]);
-    mma_f16(d0, lo, b[0], b[1]);
-    mma_f16(d1, lo, b[2], b[3]);
-    mma_f16(d0, hi, b[0], b[1]);
-    mma_f16(d1, hi, b[2], b[3]);
-}
+// A 16 x 16 block (ib, jb) of a strip matrix as B operands (rows i = columns of the result), and the product
+// planes x block in two tiles of accumulators, in three rounds.
+struct Block {
+    uint32_t hi[4], lo[4];
+    float d0[4], d1[4];
+    __device__ __forceinline__ void load(const __half* strips, int ib, int jb, int lane) {
+        const __half* at = strips + strip_base(ib) + ((lane & 7) + (lane >> 4) * 8) * strip_ld(ib) + 16 * jb + ((lane >> 3) & 1) * 8;
+        ldsm4(lo, at + 16 * strip_ld(ib));
+        ldsm4(hi, at);
+#pragma unroll
+        for (int c = 0; c < 4; c++) d0[c] = d1[c] = 0.f;
+    }
+    __device__ __forceinline__ void round(int r, const uint32_t (&ah)[4], const uint32_t (&al)[4]) {
+        mma_f16(d0, r == 1 ? al : ah, r == 0 ? lo[0] : hi[0], r == 0 ? lo[1] : hi[1]);
+        mma_f16(d1, r == 1 ? al : ah, r == 0 ? lo[2] : hi[2], r == 0 ? lo[3] : hi[3]);
+    }
+};
 
 // One chunk's step of 16 state rows, by one warp: S (rows row0 + g and + 8, columns 8 n + 2 t, + 1) to the
 // state after it, with outputs where kOut.  vp and op: v and out at (row 0, this thread's first state row).
@@ -521,14 +541,14 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
 #pragma unroll
         for (int c = 0; c < 4; c++) X[n][c] = O[n][c] = 0.f;
     {
-        float m0 = 0.f, m1 = 0.f;
+        float m[2][4] = {};   // several chains of maxima, joined at the end
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            m0 = amax(amax(m0, S[n][0]), S[n][1]);
-            m1 = amax(amax(m1, S[n][2]), S[n][3]);
-        }
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) m[c >> 1][(2 * n + c) & 3] = amax(m[c >> 1][(2 * n + c) & 3], S[n][c]);
         float sv0, sv1;
-        const float p0 = row_pow(quad_max(m0), sv0), p1 = row_pow(quad_max(m1), sv1);
+        const float p0 = row_pow(quad_max(fmaxf(fmaxf(m[0][0], m[0][1]), fmaxf(m[0][2], m[0][3]))), sv0);
+        const float p1 = row_pow(quad_max(fmaxf(fmaxf(m[1][0], m[1][1]), fmaxf(m[1][2], m[1][3]))), sv1);
         const int brow = (lane & 7) + (lane >> 4) * 8, bcol = ((lane >> 3) & 1) * 8;
 #pragma unroll
         for (int ks = 0; ks < DK / 16; ks++) {
@@ -537,31 +557,46 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
             split2(S[2 * ks][2] * p1, S[2 * ks][3] * p1, hi[1], lo[1]);
             split2(S[2 * ks + 1][0] * p0, S[2 * ks + 1][1] * p0, hi[2], lo[2]);
             split2(S[2 * ks + 1][2] * p1, S[2 * ks + 1][3] * p1, hi[3], lo[3]);
+            // each round touches every accumulator once, so no product waits for the one before it
+            uint32_t bk[kNB][4], bq[kNB][4];
 #pragma unroll
             for (int nn = 0; nn < kNB; nn++) {
-                const int off = (nn * 16 + brow) * LD + ks * 16 + bcol;
-                uint32_t b[4];
-                if (KP == 2) {
-                    ldsm4(b, &sm.k[KP - 1][off]);
-                    mma_f16(X[2 * nn], hi, b[0], b[1]);
-                    mma_f16(X[2 * nn + 1], hi, b[2], b[3]);
-                }
-                ldsm4(b, &sm.k[0][off]);
-                mma_f16(X[2 * nn], lo, b[0], b[1]);
-                mma_f16(X[2 * nn + 1], lo, b[2], b[3]);
-                mma_f16(X[2 * nn], hi, b[0], b[1]);
-                mma_f16(X[2 * nn + 1], hi, b[2], b[3]);
+                ldsm4(bk[nn], &sm.k[0][(nn * 16 + brow) * LD + ks * 16 + bcol]);
+                if (kOut) ldsm4(bq[nn], &sm.q[0][(nn * 16 + brow) * LD + ks * 16 + bcol]);
+            }
+#pragma unroll
+            for (int nn = 0; nn < kNB; nn++) {
+                mma_f16(X[2 * nn], lo, bk[nn][0], bk[nn][1]);
+                mma_f16(X[2 * nn + 1], lo, bk[nn][2], bk[nn][3]);
                 if (kOut) {
-                    if (KP == 2) {
-                        ldsm4(b, &sm.q[KP - 1][off]);
-                        mma_f16(O[2 * nn], hi, b[0], b[1]);
-                        mma_f16(O[2 * nn + 1], hi, b[2], b[3]);
+                    mma_f16(O[2 * nn], lo, bq[nn][0], bq[nn][1]);
+                    mma_f16(O[2 * nn + 1], lo, bq[nn][2], bq[nn][3]);
+                }
+            }
+            if (KP == 2) {
+                uint32_t wk[kNB][4], wq[kNB][4];
+#pragma unroll
+                for (int nn = 0; nn < kNB; nn++) {
+                    ldsm4(wk[nn], &sm.k[KP - 1][(nn * 16 + brow) * LD + ks * 16 + bcol]);
+                    if (kOut) ldsm4(wq[nn], &sm.q[KP - 1][(nn * 16 + brow) * LD + ks * 16 + bcol]);
+                }
+#pragma unroll
+                for (int nn = 0; nn < kNB; nn++) {
+                    mma_f16(X[2 * nn], hi, wk[nn][0], wk[nn][1]);
+                    mma_f16(X[2 * nn + 1], hi, wk[nn][2], wk[nn][3]);
+                    if (kOut) {
+                        mma_f16(O[2 * nn], hi, wq[nn][0], wq[nn][1]);
+                        mma_f16(O[2 * nn + 1], hi, wq[nn][2], wq[nn][3]);
                     }
-                    ldsm4(b, &sm.q[0][off]);
-                    mma_f16(O[2 * nn], lo, b[0], b[1]);
-                    mma_f16(O[2 * nn + 1], lo, b[2], b[3]);
-                    mma_f16(O[2 * nn], hi, b[0], b[1]);
-                    mma_f16(O[2 * nn + 1], hi, b[2], b[3]);
+                }
+            }
+#pragma unroll
+            for (int nn = 0; nn < kNB; nn++) {
+                mma_f16(X[2 * nn], hi, bk[nn][0], bk[nn][1]);
+                mma_f16(X[2 * nn + 1], hi, bk[nn][2], bk[nn][3]);
+                if (kOut) {
+                    mma_f16(O[2 * nn], hi, bq[nn][0], bq[nn][1]);
+                    mma_f16(O[2 * nn + 1], hi, bq[nn][2], bq[nn][3]);
                 }
             }
         }
@@ -577,46 +612,64 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
             }
     }
     // U in the place of R; O_i += P_ij U_j
+    static_assert(kNB == 2, "two blocks of 16 tokens");
     uint32_t uh[kNB][4], ul[kNB][4];
+    {
+        float inv[kNB][2];
+        Block d[kNB];
 #pragma unroll
-    for (int i = 0; i < kNB; i++) {
-        float inv[2], d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-        to_planes(X[2 * i], X[2 * i + 1], uh[i], ul[i], inv);
-        mma_block(d0, d1, uh[i], ul[i], sm.m, i, i, lane);
-        const float db = sm.dscale[i];
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            X[2 * i][c] = d0[c] * (db * inv[c >> 1]);
-            X[2 * i + 1][c] = d1[c] * (db * inv[c >> 1]);
+        for (int i = 0; i < kNB; i++) {
+            d[i].load(sm.m, i, i, lane);
+            to_planes(X[2 * i], X[2 * i + 1], uh[i], ul[i], inv[i]);
         }
-    }
 #pragma unroll
-    for (int j = 0; j < kNB; j++) {
-        float us[2];
-        to_planes(X[2 * j], X[2 * j + 1], uh[j], ul[j], us);
+        for (int r = 0; r < 3; r++)
 #pragma unroll
-        for (int i = j + 1; i < kNB; i++) {
-            float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_block(d0, d1, uh[j], ul[j], sm.m, i, j, lane);
-            const float b = -sm.bscale;
+            for (int i = 0; i < kNB; i++) d[i].round(r, uh[i], ul[i]);
+#pragma unroll
+        for (int i = 0; i < kNB; i++) {
+            const float db = sm.dscale[i];
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                X[2 * i][c] = fmaf(b * us[c >> 1], d0[c], X[2 * i][c]);
-                X[2 * i + 1][c] = fmaf(b * us[c >> 1], d1[c], X[2 * i + 1][c]);
+                X[2 * i][c] = d[i].d0[c] * (db * inv[i][c >> 1]);
+                X[2 * i + 1][c] = d[i].d1[c] * (db * inv[i][c >> 1]);
             }
         }
+    }
+    const auto add_out = [&](const Block& p, int i, int j, const float (&us)[2]) {
+        const float* ps = &sm.pscale[j][16 * i + 2 * t];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            O[2 * i][c] = fmaf(ps[c & 1] * us[c >> 1], p.d0[c], O[2 * i][c]);
+            O[2 * i + 1][c] = fmaf(ps[8 + (c & 1)] * us[c >> 1], p.d1[c], O[2 * i + 1][c]);
+        }
+    };
+    {
+        float us[2];
+        Block b10, p00, p10;
+        b10.load(sm.m, 1, 0, lane);
+        if (kOut) p00.load(sm.p, 0, 0, lane), p10.load(sm.p, 1, 0, lane);
+        to_planes(X[0], X[1], uh[0], ul[0], us);
+#pragma unroll
+        for (int r = 0; r < 3; r++) {
+            b10.round(r, uh[0], ul[0]);
+            if (kOut) p00.round(r, uh[0], ul[0]), p10.round(r, uh[0], ul[0]);
+        }
+        const float b = -sm.bscale;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            X[2][c] = fmaf(b * us[c >> 1], b10.d0[c], X[2][c]);
+            X[3][c] = fmaf(b * us[c >> 1], b10.d1[c], X[3][c]);
+        }
         if (kOut) {
+            add_out(p00, 0, 0, us);
+            add_out(p10, 1, 0, us);
+            Block p11;
+            p11.load(sm.p, 1, 1, lane);
+            to_planes(X[2], X[3], uh[1], ul[1], us);
 #pragma unroll
-            for (int i = j; i < kNB; i++) {
-                float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_block(d0, d1, uh[j], ul[j], sm.p, i, j, lane);
-                const float* ps = &sm.pscale[j][16 * i + 2 * t];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    O[2 * i][c] = fmaf(ps[c & 1] * us[c >> 1], d0[c], O[2 * i][c]);
-                    O[2 * i + 1][c] = fmaf(ps[8 + (c & 1)] * us[c >> 1], d1[c], O[2 * i + 1][c]);
-                }
-            }
+            for (int r = 0; r < 3; r++) p11.round(r, uh[1], ul[1]);
+            add_out(p11, 1, 1, us);
         }
     }
     if (kOut) {
@@ -652,32 +705,42 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
     const float gamma = sm.ee[kC - 1];
     const int trow = (lane & 7) + ((lane >> 3) & 1) * 8, tcol = (lane >> 4) * 8;
 #pragma unroll
-    for (int nn = 0; nn < NT / 2; nn++) {
-        float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t b[kNB][4];
+    for (int n0 = 0; n0 < NT / 2; n0 += 2) {   // 32 state columns at a time, four accumulators a round
+        float d[4][4] = {};
+        uint32_t b[kNB][2][4];
 #pragma unroll
-        for (int jb = 0; jb < kNB; jb++) {
-            const int off = (16 * jb + trow) * LD + nn * 16 + tcol;
-            if (KP == 2) {
-                uint32_t w[4];
-                ldsm4t(w, &sm.k[KP - 1][off]);
-                mma_f16(d0, uh[jb], w[0], w[1]);
-                mma_f16(d1, uh[jb], w[2], w[3]);
+        for (int jb = 0; jb < kNB; jb++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) ldsm4t(b[jb][u], &sm.k[0][(16 * jb + trow) * LD + (n0 + u) * 16 + tcol]);
+#pragma unroll
+        for (int jb = 0; jb < kNB; jb++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                mma_f16(d[2 * u], ul[jb], b[jb][u][0], b[jb][u][1]);
+                mma_f16(d[2 * u + 1], ul[jb], b[jb][u][2], b[jb][u][3]);
             }
-            ldsm4t(b[jb], &sm.k[0][off]);
-            mma_f16(d0, ul[jb], b[jb][0], b[jb][1]);
-            mma_f16(d1, ul[jb], b[jb][2], b[jb][3]);
+        if (KP == 2) {
+#pragma unroll
+            for (int jb = 0; jb < kNB; jb++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    uint32_t w[4];
+                    ldsm4t(w, &sm.k[KP - 1][(16 * jb + trow) * LD + (n0 + u) * 16 + tcol]);
+                    mma_f16(d[2 * u], uh[jb], w[0], w[1]);
+                    mma_f16(d[2 * u + 1], uh[jb], w[2], w[3]);
+                }
         }
 #pragma unroll
-        for (int jb = 0; jb < kNB; jb++) {
-            mma_f16(d0, uh[jb], b[jb][0], b[jb][1]);
-            mma_f16(d1, uh[jb], b[jb][2], b[jb][3]);
-        }
+        for (int jb = 0; jb < kNB; jb++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            S[2 * nn][c] = fmaf(gamma, S[2 * nn][c], (c < 2 ? iv0 : iv1) * d0[c]);
-            S[2 * nn + 1][c] = fmaf(gamma, S[2 * nn + 1][c], (c < 2 ? iv0 : iv1) * d1[c]);
-        }
+            for (int u = 0; u < 2; u++) {
+                mma_f16(d[2 * u], uh[jb], b[jb][u][0], b[jb][u][1]);
+                mma_f16(d[2 * u + 1], uh[jb], b[jb][u][2], b[jb][u][3]);
+            }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) S[2 * n0 + u][c] = fmaf(gamma, S[2 * n0 + u][c], (c < 2 ? iv0 : iv1) * d[u][c]);
     }
 }
 
@@ -753,7 +816,7 @@ __global__ void __launch_bounds__(ChunkCfg<DK, T, kWide>::kThreads, ChunkCfg<DK,
     if constexpr (kWide) {
         if (warp < 4) {
             Source<DK, T, kOut> in;
-            in.init(a, t0, h, hq);
+            in.init(a, t0, h, hq, blockIdx.x * Cfg::kRows, Cfg::kRows);
             if (t0 < t1) in.stage(sm.raw, chunk_len(t0));
             for (uint64_t at = t0, n = 0; at < t1; at += kC, n++) {
                 prepare_chunk<DK, T, kOut>(sm.c[n & 1], sm.raw, a, in, chunk_len(at));
@@ -768,7 +831,7 @@ __global__ void __launch_bounds__(ChunkCfg<DK, T, kWide>::kThreads, ChunkCfg<DK,
         }
     } else {
         Source<DK, T, kOut> in;
-        in.init(a, t0, h, hq);
+        in.init(a, t0, h, hq, blockIdx.x * Cfg::kRows, Cfg::kRows);
         if (t0 < t1) in.stage(sm.raw, chunk_len(t0));
         for (uint64_t at = t0; at < t1; at += kC) {
             prepare_chunk<DK, T, kOut>(sm.c[0], sm.raw, a, in, chunk_len(at));
