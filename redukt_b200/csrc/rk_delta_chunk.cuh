@@ -50,7 +50,10 @@ struct ChunkCfg {
     static constexpr int LD = DK + 8;           // halves per row of a plane
     static constexpr int kThreads = kWide ? 384 : 128;
     static constexpr int kRows = kWide ? 128 : 64;   // state rows per block
-    static constexpr int kMinBlocks = kWide ? 1 : DK == 64 ? 4 : kF32 ? 2 : 3;   // what registers and shared memory allow
+    // Resident blocks: what shared memory and 168 registers allow.  With key size 64 a fourth block would fit
+    // at 128 registers, but costs more by spills than it brings: 32 windows of 2,700 f32 tokens take
+    // 0.72 ms at three blocks, 0.85 ms at four, 1.04 ms at two.
+    static constexpr int kMinBlocks = kWide ? 1 : DK == 128 && kF32 ? 2 : 3;
 };
 
 // A prepared chunk.
@@ -109,15 +112,32 @@ __device__ __forceinline__ float quad_max(float m) {
     return fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
 }
 
-// two scaled values as one register of each plane
-__device__ __forceinline__ uint32_t pack_hi(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
+// Two f32 values at once (packed arithmetic): x * a + y elementwise, and x * a.
+__device__ __forceinline__ float2 fma2(float2 x, float2 a, float2 y) {
+    float2 r;
+    asm("{\n\t.reg .b64 p, q, s;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 s, {%6, %7};\n\t"
+        "fma.rn.f32x2 p, p, q, s;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(a.x), "f"(a.y), "f"(y.x), "f"(y.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 x, float2 a) {
+    float2 r;
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(a.x), "f"(a.y));
+    return r;
+}
+
+// two values, times s, as one register of each plane
+__device__ __forceinline__ uint32_t pack_hi(float x, float y, float s) {
+    const float2 v = mul2(make_float2(x, y), make_float2(s, s));
+    const __half2 h = __floats2half2_rn(v.x, v.y);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+__device__ __forceinline__ void split2(float x, float y, float s, uint32_t& hi, uint32_t& lo) {
+    const float2 v = mul2(make_float2(x, y), make_float2(s, s));
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    const float2 w = fma2(__half22float2(h), make_float2(-1.f, -1.f), v);
+    const __half2 l = __floats2half2_rn(w.x, w.y);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -191,8 +211,8 @@ struct RowLoad {
             uint32_t h[N / 2], w[N / 2];
 #pragma unroll
             for (int c = 0; c < N / 2; c++) {
-                if constexpr (sizeof(T) == 4) split2(s * get(i, 2 * c), s * get(i, 2 * c + 1), h[c], w[c]);
-                else h[c] = pack_hi(s * get(i, 2 * c), s * get(i, 2 * c + 1));
+                if constexpr (sizeof(T) == 4) split2(get(i, 2 * c), get(i, 2 * c + 1), s, h[c], w[c]);
+                else h[c] = pack_hi(get(i, 2 * c), get(i, 2 * c + 1), s);
             }
             const int at = (l + 8 * i) * N;
             if constexpr (sizeof(T) == 4) {
@@ -431,10 +451,10 @@ __device__ __forceinline__ void prepare_chunk(Chunk<DK, T>& sm, const uint4* raw
         for (int n = 0; n < 2; n++) {
             const int at = g * ld + 16 * nb + 8 * n + 2 * t;
             uint32_t x, y;
-            split2(acc[s][n][0] * p0, acc[s][n][1] * p0, x, y);
+            split2(acc[s][n][0], acc[s][n][1], p0, x, y);
             *reinterpret_cast<uint32_t*>(hi + at) = x;
             *reinterpret_cast<uint32_t*>(lo + at) = y;
-            split2(acc[s][n][2] * p1, acc[s][n][3] * p1, x, y);
+            split2(acc[s][n][2], acc[s][n][3], p1, x, y);
             *reinterpret_cast<uint32_t*>(hi + at + 8 * ld) = x;
             *reinterpret_cast<uint32_t*>(lo + at + 8 * ld) = y;
         }
@@ -493,10 +513,10 @@ __device__ __forceinline__ void to_planes(const float (&x)[4], const float (&y)[
         m1 = amax(amax(m1, x[2 + c]), y[2 + c]);
     }
     const float s0 = row_pow(quad_max(m0), inv[0]), s1 = row_pow(quad_max(m1), inv[1]);
-    split2(x[0] * s0, x[1] * s0, hi[0], lo[0]);
-    split2(x[2] * s1, x[3] * s1, hi[1], lo[1]);
-    split2(y[0] * s0, y[1] * s0, hi[2], lo[2]);
-    split2(y[2] * s1, y[3] * s1, hi[3], lo[3]);
+    split2(x[0], x[1], s0, hi[0], lo[0]);
+    split2(x[2], x[3], s1, hi[1], lo[1]);
+    split2(y[0], y[1], s0, hi[2], lo[2]);
+    split2(y[2], y[3], s1, hi[3], lo[3]);
 }
 
 // d0, d1 (16 columns) += planes x a 16 x 16 block of a strip matrix (rows i = columns of the result)
@@ -553,10 +573,10 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
 #pragma unroll
         for (int ks = 0; ks < DK / 16; ks++) {
             uint32_t hi[4], lo[4];
-            split2(S[2 * ks][0] * p0, S[2 * ks][1] * p0, hi[0], lo[0]);
-            split2(S[2 * ks][2] * p1, S[2 * ks][3] * p1, hi[1], lo[1]);
-            split2(S[2 * ks + 1][0] * p0, S[2 * ks + 1][1] * p0, hi[2], lo[2]);
-            split2(S[2 * ks + 1][2] * p1, S[2 * ks + 1][3] * p1, hi[3], lo[3]);
+            split2(S[2 * ks][0], S[2 * ks][1], p0, hi[0], lo[0]);
+            split2(S[2 * ks][2], S[2 * ks][3], p1, hi[1], lo[1]);
+            split2(S[2 * ks + 1][0], S[2 * ks + 1][1], p0, hi[2], lo[2]);
+            split2(S[2 * ks + 1][2], S[2 * ks + 1][3], p1, hi[3], lo[3]);
             // each round touches every accumulator once, so no product waits for the one before it
             uint32_t bk[kNB][4], bq[kNB][4];
 #pragma unroll
@@ -697,10 +717,10 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
     const float q0 = row_pow(quad_max(n0), iv0), q1 = row_pow(quad_max(n1), iv1);
 #pragma unroll
     for (int jb = 0; jb < kNB; jb++) {
-        split2(X[2 * jb][0] * q0, X[2 * jb][1] * q0, uh[jb][0], ul[jb][0]);
-        split2(X[2 * jb][2] * q1, X[2 * jb][3] * q1, uh[jb][1], ul[jb][1]);
-        split2(X[2 * jb + 1][0] * q0, X[2 * jb + 1][1] * q0, uh[jb][2], ul[jb][2]);
-        split2(X[2 * jb + 1][2] * q1, X[2 * jb + 1][3] * q1, uh[jb][3], ul[jb][3]);
+        split2(X[2 * jb][0], X[2 * jb][1], q0, uh[jb][0], ul[jb][0]);
+        split2(X[2 * jb][2], X[2 * jb][3], q1, uh[jb][1], ul[jb][1]);
+        split2(X[2 * jb + 1][0], X[2 * jb + 1][1], q0, uh[jb][2], ul[jb][2]);
+        split2(X[2 * jb + 1][2], X[2 * jb + 1][3], q1, uh[jb][3], ul[jb][3]);
     }
     const float gamma = sm.ee[kC - 1];
     const int trow = (lane & 7) + ((lane >> 3) & 1) * 8, tcol = (lane >> 4) * 8;
@@ -740,7 +760,13 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
 #pragma unroll
         for (int u = 0; u < 4; u++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) S[2 * n0 + u][c] = fmaf(gamma, S[2 * n0 + u][c], (c < 2 ? iv0 : iv1) * d[u][c]);
+            for (int c = 0; c < 4; c += 2) {
+                const float iv = c ? iv1 : iv0;
+                float(&x)[4] = S[2 * n0 + u];
+                const float2 r = fma2(make_float2(gamma, gamma), make_float2(x[c], x[c + 1]),
+                                      mul2(make_float2(iv, iv), make_float2(d[u][c], d[u][c + 1])));
+                x[c] = r.x, x[c + 1] = r.y;
+            }
     }
 }
 
