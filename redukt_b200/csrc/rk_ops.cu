@@ -52,7 +52,7 @@ Device g_device[kMaxDevices];
 
 template <int BN, class T>
 cudaError_t set_smem() {
-    return cudaFuncSetAttribute(rk::w8::k_w8a8_tc<BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rk::w8::tc_smem<BN>());
+    return cudaFuncSetAttribute(rk::w8::k_w8a8_tc<BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rk::w8::kSmemMax);
 }
 
 template <int DK, class T, bool kWide>
@@ -228,7 +228,7 @@ int32_t tensor_map(CUtensorMap* map, const Device& d, CUtensorMapDataType type, 
     const cuuint64_t dims[2] = {width, rows}, strides[1] = {ld * elem};
     const cuuint32_t box[2] = {(cuuint32_t)(128 / elem), box_rows}, one[2] = {1, 1};
     const CUresult r = d.encode(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_err("cuTensorMapEncodeTiled failed (%d) for %llu x %llu at stride %llu", (int)r, (unsigned long long)rows,
                 (unsigned long long)width, (unsigned long long)ld);
@@ -241,7 +241,8 @@ template <int BN, class T>
 int32_t launch_tc(const Device& d, const rk::w8::Args& a, cudaStream_t st, bool after_quant) {
     using namespace rk::w8;
     CUtensorMap ma, mw, mo;
-    if (int32_t rc = tensor_map(&ma, d, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.a, a.k, a.m, a.ld_a, kTileM)) return rc;
+    const uint32_t rows_a = (uint32_t)std::min<uint64_t>(kTileM, ceil_div(a.m, 8) * 8);
+    if (int32_t rc = tensor_map(&ma, d, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.a, a.k, a.m, a.ld_a, rows_a)) return rc;
     if (int32_t rc = tensor_map(&mw, d, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.k, a.n, a.ld_w, BN)) return rc;
     const bool tma_out = aligned(a.out, 16) && a.ld_o * sizeof(T) % 16 == 0;
     if (tma_out) {
@@ -250,11 +251,11 @@ int32_t launch_tc(const Device& d, const rk::w8::Args& a, cudaStream_t st, bool 
     } else {
         mo = ma;   // never used
     }
-    TcArgs g = {a.as, a.ws, a.out, a.ld_o, a.m, a.n, a.k, (uint32_t)ceil_div(a.m, kTileM), (uint32_t)ceil_div(a.n, BN), tma_out, d.err};
+    TcArgs g = {a.as, a.ws, a.out, a.ld_o, a.m, a.n, a.k, (uint32_t)ceil_div(a.m, kTileM), (uint32_t)ceil_div(a.n, BN), rows_a, stages<BN>(rows_a), tma_out, d.err};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)std::min<uint64_t>((uint64_t)g.tiles_m * g.tiles_n, d.sms));
     cfg.blockDim = dim3(kTcThreads);
-    cfg.dynamicSmemBytes = tc_smem<BN>();
+    cfg.dynamicSmemBytes = kSmemMax;
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -265,8 +266,9 @@ int32_t launch_tc(const Device& d, const rk::w8::Args& a, cudaStream_t st, bool 
     return BACKEND_OK;
 }
 
-// Width of the tensor-core tile: the one whose waves over the SMs cost least, a tile of BN channels
-// taking about as long as BN + 32 (its fill and drain do not shrink with it).
+// Width of the tensor-core tile: the one whose waves over the SMs cost least, a tile of BN channels taking as
+// long as BN + 32 (its fill and drain do not shrink with it, and a narrow tile reads more shared memory per
+// product).
 int tile_width(uint64_t m, uint64_t n, int sms) {
     int best = 256;
     uint64_t least = ~0ull;
@@ -280,8 +282,36 @@ int tile_width(uint64_t m, uint64_t n, int sms) {
     return best;
 }
 
+template <int M, class X, class T>
+int32_t launch_few(const Device& d, const rk::w8::Args& a, const X* x, uint64_t ld_x, cudaStream_t st, bool after_quant) {
+    using namespace rk::w8;
+    // warps along K: as many as it takes to put two blocks on every SM, with two K steps left for each
+    const uint64_t groups = ceil_div(a.n, 16), steps = ceil_div(a.k, 64);
+    int wk = 1;
+    while (wk < kFewWarps && groups * wk < 2ull * kFewWarps * d.sms && steps >= 4ull * wk) wk *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ceil_div(groups, kFewWarps / wk));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = sizeof(X) > 1 ? M * steps * 64 : 0;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = after_quant ? 1 : 0;
+    OP_CK(cudaLaunchKernelEx(&cfg, k_w8a8_few<M, X, T>, a, x, ld_x, wk));
+    return BACKEND_OK;
+}
+
+template <class X, class T>
+int32_t few(const Device& d, const rk::w8::Args& a, const X* x, uint64_t ld_x, cudaStream_t st, bool after_quant) {
+    if (a.m <= 1) return launch_few<1, X, T>(d, a, x, ld_x, st, after_quant);
+    return launch_few<2, X, T>(d, a, x, ld_x, st, after_quant);
+}
+
 template <class T>
 int32_t matmul_t(const Device& d, const rk::w8::Args& a, cudaStream_t st, bool after_quant) {
+    if (a.m <= rk::w8::kFewTokens) return few<int8_t, T>(d, a, nullptr, 0, st, after_quant);
     switch (tile_width(a.m, a.n, d.sms)) {
         case 256: return launch_tc<256, T>(d, a, st, after_quant);
         case 128: return launch_tc<128, T>(d, a, st, after_quant);
@@ -436,6 +466,14 @@ int32_t redukt_b200_w8a8_linear(const void* d_x, int32_t dtype, uint32_t n_token
     Device* d = nullptr;
     if (int32_t rc = device(&d)) return rc;
     const cudaStream_t st = stream_of(cuda_stream);
+    if (n_tokens <= rk::w8::kFewTokens && (uint64_t)n_tokens * k <= rk::w8::kFewFused) {
+        const rk::w8::Args a = {nullptr, nullptr, d_w, d_w_scale, 0, ld_w, ld_out, n_tokens, n_out, k, d_out};
+        if (dtype == REDUKT_DTYPE_F32)
+            return out_dtype == REDUKT_DTYPE_F32 ? few<float, float>(*d, a, (const float*)d_x, ld_x, st, false)
+                                                 : few<float, __nv_bfloat16>(*d, a, (const float*)d_x, ld_x, st, false);
+        return out_dtype == REDUKT_DTYPE_F32 ? few<__nv_bfloat16, float>(*d, a, (const __nv_bfloat16*)d_x, ld_x, st, false)
+                                             : few<__nv_bfloat16, __nv_bfloat16>(*d, a, (const __nv_bfloat16*)d_x, ld_x, st, false);
+    }
     if (int32_t rc = quantize(d_x, dtype, n_tokens, k, ld_x, q, quant_ld(k), s, st)) return rc;
     rk::w8::Args a = {q, s, d_w, d_w_scale, quant_ld(k), ld_w, ld_out, n_tokens, n_out, k, d_out};
     return matmul(*d, a, out_dtype, st, true);

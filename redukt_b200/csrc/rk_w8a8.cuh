@@ -120,40 +120,117 @@ struct Args {
     void* out;
 };
 
-// 64 x 64 outputs per block, 4 x 4 per thread, dp4a over K in steps of 64 bytes.
-template <class T>
-__global__ void __launch_bounds__(256) k_w8a8_dp4a(Args a) {
-    __shared__ int sa[64][17], sw[64][17];
-    const uint32_t n0 = blockIdx.x * 64, m0 = blockIdx.y * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (uint32_t k0 = 0; k0 < a.k; k0 += 64) {
-        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-            const uint32_t r = i >> 4, c = k0 + (i & 15) * 4;
-            uint32_t va = 0, vw = 0;
-            for (int j = 0; j < 4; j++) {
-                if (c + j >= a.k) break;
-                if (m0 + r < a.m) va |= (uint32_t)(uint8_t)a.a[(m0 + r) * a.ld_a + c + j] << (8 * j);
-                if (n0 + r < a.n) vw |= (uint32_t)(uint8_t)a.w[(n0 + r) * a.ld_w + c + j] << (8 * j);
-            }
-            sa[r][i & 15] = (int)va;
-            sw[r][i & 15] = (int)vw;
-        }
+// ---- one or two tokens: the weights stream past ----
+//
+// Bound by the weights' bytes.  A warp takes 16 channels and a share of K; lane (g, t) reads 16 bytes at 16 t
+// of rows g and g + 8 in steps of 64 bytes and adds the dot products with each token's 16 bytes (dp4a).
+// The four lanes of a row, then the warps that share channels, add their exact int32 sums.  A 65,536 x 768
+// head takes 11.3 us for one token (the tensor-core tiles 16 us), 17.5 us for four (16 us): dp4a does
+// not keep up with the weights beyond two, and warp-level int8 mma does so even less (18 us at one).
+// Where the activations are small each block quantises them itself into shared memory while its first
+// weights are on their way, which saves the quantiser's launch; otherwise they are read as int8.
+constexpr int kFewThreads = 256, kFewWarps = 8, kFewDepth = 4;
+constexpr uint32_t kFewTokens = 2;
+constexpr uint32_t kFewFused = 16384;   // most activations a block quantises itself
+
+__device__ __forceinline__ uint4 load_once(const int8_t* p) {   // weights are read once: not kept in L1
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ int dot16(uint4 w, uint4 x, int acc) {
+    acc = __dp4a((int)w.x, (int)x.x, acc);
+    acc = __dp4a((int)w.y, (int)x.y, acc);
+    acc = __dp4a((int)w.z, (int)x.z, acc);
+    return __dp4a((int)w.w, (int)x.w, acc);
+}
+
+// grid: ceil(n / (16 * kFewWarps / wk)); wk warps (a divisor of 8) share each 16 channels.  X: the activations'
+// type, int8_t = already quantised (a.a, a.as).
+template <int M, class X, class T>
+__global__ void __launch_bounds__(kFewThreads) k_w8a8_few(Args a, const X* __restrict__ x, uint64_t ld_x, int wk) {
+    constexpr bool kFused = sizeof(X) > 1;
+    extern __shared__ uint4 sx[];                     // fused: [M][steps * 4] vectors of int8
+    __shared__ int part[kFewWarps][M][16];
+    __shared__ float top[kFewWarps], scale[M];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int wn = kFewWarps / wk, kw = warp % wk;
+    const uint32_t n0 = (blockIdx.x * wn + warp / wk) * 16;
+    const int steps = (int)((a.k + 63) / 64);
+    const int8_t* w0 = a.w + (uint64_t)min(n0 + g, a.n - 1) * a.ld_w + 16 * t;
+    const int8_t* w1 = a.w + (uint64_t)min(n0 + g + 8, a.n - 1) * a.ld_w + 16 * t;
+    uint4 w[kFewDepth][2];
+    const auto fetch = [&](uint4(&dst)[2], int s) {
+        const bool live = s < steps && (uint32_t)(64 * s + 16 * t) < a.k;
+        dst[0] = live ? load_once(w0 + 64 * s) : make_uint4(0, 0, 0, 0);
+        dst[1] = live ? load_once(w1 + 64 * s) : make_uint4(0, 0, 0, 0);
+    };
+#pragma unroll
+    for (int d = 0; d < kFewDepth; d++) fetch(w[d], kw + d * wk);
+    if constexpr (kFused) {
+        constexpr int kPer = kFewThreads / M;         // threads per token
+        const uint32_t tok = threadIdx.x / kPer, i0 = threadIdx.x % kPer;
+        const X* xr = x + (uint64_t)min(tok, a.m - 1) * ld_x;
+        float m = 0.f;
+        for (uint32_t i = i0; i < a.k; i += kPer) m = fmaxf(m, fabsf(to_f32(xr[i])));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        if (lane == 0) top[warp] = m;
         __syncthreads();
 #pragma unroll
-        for (int c = 0; c < 16; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = __dp4a(sa[ty + 16 * i][c], sw[tx + 16 * j][c], acc[i][j]);
+        for (int q = 0; q < kPer / 32; q++) m = fmaxf(m, top[tok * (kPer / 32) + q]);
+        const float s = row_scale(m), inv = __fdiv_rn(1.f, s);
+        if (i0 == 0) scale[tok] = s;
+        int8_t* row = reinterpret_cast<int8_t*>(sx + tok * steps * 4);
+        for (uint32_t i = i0; i < (uint32_t)steps * 64; i += kPer) row[i] = i < a.k && tok < a.m ? (int8_t)quant_one(to_f32(xr[i]), inv) : (int8_t)0;
         __syncthreads();
+    } else {
+        tc::grid_wait();
     }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            const uint32_t r = m0 + ty + 16 * i, c = n0 + tx + 16 * j;
-            if (r < a.m && c < a.n)
-                put((T*)a.out + r * a.ld_o + c, __fmul_rn((float)acc[i][j], __fmul_rn(a.ws[c], a.as[r])));
+    int acc[M][2] = {};
+    for (int s0 = kw; s0 < steps; s0 += kFewDepth * wk) {
+#pragma unroll
+        for (int d = 0; d < kFewDepth; d++) {
+            const int s = s0 + d * wk;
+            if (s >= steps) break;
+            const int left = (int)a.k - (64 * s + 16 * t);   // bytes of this lane's vector that are data
+#pragma unroll
+            for (int j = 0; j < M; j++) {
+                uint4 b = make_uint4(0, 0, 0, 0);
+                if constexpr (kFused) {
+                    b = sx[(j * steps + s) * 4 + t];
+                } else if (j < (int)a.m && left > 0) {
+                    b = *reinterpret_cast<const uint4*>(a.a + (uint64_t)j * a.ld_a + 64 * s + 16 * t);
+                    if (left < 16) {   // what lies past K is not data
+                        uint32_t* q = reinterpret_cast<uint32_t*>(&b);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) q[c] = left >= 4 * c + 4 ? q[c] : left > 4 * c ? q[c] & ((1u << (8 * (left - 4 * c))) - 1) : 0u;
+                    }
+                }
+                acc[j][0] = dot16(w[d][0], b, acc[j][0]);
+                acc[j][1] = dot16(w[d][1], b, acc[j][1]);
+            }
+            fetch(w[d], s + kFewDepth * wk);
         }
+    }
+#pragma unroll
+    for (int j = 0; j < M; j++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            int v = acc[j][i];
+            v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+            v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+            if (t == 0) part[warp][j][g + 8 * i] = v;
+        }
+    __syncthreads();
+    for (int e = threadIdx.x; e < wn * M * 16; e += kFewThreads) {
+        const int ch = e % 16, grp = e / 16 % wn, tok = e / (16 * wn);
+        int sum = 0;
+        for (int q = 0; q < wk; q++) sum += part[grp * wk + q][tok][ch];
+        const uint32_t n = (blockIdx.x * wn + grp) * 16 + ch;
+        if (tok < (int)a.m && n < a.n)
+            put((T*)a.out + tok * a.ld_o + n, __fmul_rn((float)sum, __fmul_rn(a.ws[n], kFused ? scale[tok] : a.as[tok])));
+    }
 }
 
 // ---- tensor cores: 128 tokens x BN channels per tile ----
@@ -168,28 +245,36 @@ constexpr int kTileM = 128, kTileK = 128;
 constexpr int kTcThreads = 192;
 constexpr long long kWaitCycles = 4000000000ll;   // about 2 s
 
-template <int BN>
-__host__ __device__ constexpr int stages() { return BN == 256 ? 4 : BN == 128 ? 6 : 8; }
+// Stages: as many as fit beside the rest.  A batch of fewer than 128 tokens stages only its rows (the product
+// still reads 128 rows: the next stages' bytes, whose sums nobody reads), so more weights are in flight;
+// 16 x 8,192 x 8,192 with 64-channel tiles is bound by that.
+constexpr int kMaxStages = 20;
+constexpr size_t kSmemMax = 232448;
 
 template <int BN>
 struct alignas(1024) TcSmem {
-    int8_t a[stages<BN>()][kTileM * kTileK];
-    int8_t b[stages<BN>()][BN * kTileK];
     uint8_t out[4][2][32 * 128];   // each epilogue warp: two boxes of 32 rows x 128 bytes, swizzled
     float ws[BN];
-    uint64_t full[stages<BN>()], empty[stages<BN>()];
+    uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t tfull[2], tempty[2];
     uint32_t tmem;
     int abort;
+    // then, on 1,024 bytes: stages x rows_a x 128 (and up to 128 rows from the last one's start), stages x BN x 128
 };
+__host__ __device__ constexpr size_t stage_room(size_t fixed, uint32_t rows_a) { return kSmemMax - 1024 - fixed - (kTileM - rows_a) * kTileK; }
 template <int BN>
-__host__ __device__ constexpr size_t tc_smem() { return sizeof(TcSmem<BN>) + 1024; }
+__host__ __device__ constexpr int stages(uint32_t rows_a) {
+    const size_t n = stage_room(sizeof(TcSmem<BN>), rows_a) / ((rows_a + BN) * kTileK);
+    return n < kMaxStages ? (int)n : kMaxStages;
+}
 
 struct TcArgs {
     const float *as, *ws;
     void* out;
     uint64_t ld_o;
     uint32_t m, n, k, tiles_m, tiles_n;
+    uint32_t rows_a;    // rows of an activation box: 128, or fewer (a multiple of 8) where the batch has fewer
+    int stages;
     int tma_out;        // the output can be stored by TMA (16-byte aligned rows)
     uint32_t* err;
 };
@@ -240,14 +325,15 @@ k_w8a8_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     extern __shared__ uint8_t raw[];
     using S = TcSmem<BN>;
     S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    constexpr int ST = stages<BN>();
-    constexpr uint32_t kStage = (kTileM + BN) * kTileK;
+    const uint32_t ST = (uint32_t)g.stages, a_bytes = g.rows_a * kTileK;
+    int8_t* const sa = reinterpret_cast<int8_t*>(&sm + 1);
+    int8_t* const sb = sa + ST * a_bytes + (kTileM - g.rows_a) * kTileK;
     constexpr uint32_t kCols = 2 * BN < 32 ? 32 : 2 * BN;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t kb = (g.k + kTileK - 1) / kTileK, tiles = g.tiles_m * g.tiles_n;
     volatile int* abort = &sm.abort;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < ST; i++) {
+        for (uint32_t i = 0; i < ST; i++) {
             tc::mbar_init(&sm.full[i], 1);
             tc::mbar_init(&sm.empty[i], 1);
         }
@@ -266,64 +352,80 @@ k_w8a8_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = sm.tmem;
-    tc::grid_wait();   // the activations may come from the preceding kernel
 
-    if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-                uint32_t tm, tn;
-                tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
-                for (uint32_t j = 0; j < kb; j++, it++) {
-                    const uint32_t s = it % ST;
-                    if (!wait_bar(&sm.empty[s], ((it / ST) & 1) ^ 1, abort)) {
-                        ok = false;
-                        break;
-                    }
-                    tc::mbar_expect_tx(&sm.full[s], kStage);
-                    tc::tma_load_2d(sm.a[s], &map_a, (int)(j * kTileK), (int)(tm * kTileM), &sm.full[s]);
-                    tc::tma_load_2d(sm.b[s], &map_w, (int)(j * kTileK), (int)(tn * BN), &sm.full[s]);
-                }
+    if (warp == 0) {   // the whole warp runs the loop and waits, one lane issues
+        const uint32_t stage_bytes = (g.rows_a + BN) * kTileK;
+        uint32_t it = 0, s = 0, ph = 0, tm, tn;
+        bool ok = true;
+        // the first weights do not wait for the preceding kernel; the activations may be its output
+        const uint32_t early = min(kb, ST);
+        tile_at(blockIdx.x, g.tiles_m, g.tiles_n, tm, tn);
+        for (uint32_t j = 0; j < early; j++) {
+            if (tc::elect_one()) {
+                tc::mbar_expect_tx(&sm.full[j], stage_bytes);
+                tc::tma_load_2d(sb + j * BN * kTileK, &map_w, (int)(j * kTileK), (int)(tn * BN), &sm.full[j]);
             }
-            if (!ok)   // the copies in flight land before the shared memory goes away
-                for (uint32_t i = it > ST ? it - ST : 0; i < it; i++) drain_bar(&sm.full[i % ST], (i / ST) & 1);
+            __syncwarp();
         }
-        __syncwarp();
-    } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
-            uint32_t it = 0, n = 0;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, n++) {
-                const uint32_t buf = n & 1;
-                if (!wait_bar(&sm.tempty[buf], ((n >> 1) & 1) ^ 1, abort)) break;
-                tc::tc_fence_after();
-                const uint32_t d = tmem + buf * BN;
-                for (uint32_t j = 0; j < kb; j++, it++) {
-                    const uint32_t s = it % ST;
-                    if (!wait_bar(&sm.full[s], (it / ST) & 1, abort)) {
-                        ok = false;
-                        break;
+        tc::grid_wait();
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
+            for (uint32_t j = 0; j < kb; j++, it++, s = s + 1 == ST ? (ph ^= 1, 0) : s + 1) {
+                const bool fill = it >= early;
+                if (fill && !wait_bar(&sm.empty[s], ph ^ 1, abort)) {
+                    ok = false;
+                    break;
+                }
+                if (tc::elect_one()) {
+                    if (fill) {
+                        tc::mbar_expect_tx(&sm.full[s], stage_bytes);
+                        tc::tma_load_2d(sb + s * BN * kTileK, &map_w, (int)(j * kTileK), (int)(tn * BN), &sm.full[s]);
                     }
-                    tc::tc_fence_after();
-                    const uint64_t da = sw128_desc(sm.a[s]), db = sw128_desc(sm.b[s]);
+                    tc::tma_load_2d(sa + s * a_bytes, &map_a, (int)(j * kTileK), (int)(tm * kTileM), &sm.full[s]);
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) {   // the copies in flight land before the shared memory goes away
+            for (uint32_t i = it > ST ? it - ST : 0; i < it; i++) drain_bar(&sm.full[i % ST], (i / ST) & 1);
+            __syncwarp();
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+        const uint64_t da0 = sw128_desc(sa), db0 = sw128_desc(sb);
+        uint32_t it = 0, s = 0, ph = 0, n = 0;
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, n++) {
+            const uint32_t buf = n & 1;
+            if (!wait_bar(&sm.tempty[buf], ((n >> 1) & 1) ^ 1, abort)) break;
+            tc::tc_fence_after();
+            const uint32_t d = tmem + buf * BN;
+            for (uint32_t j = 0; j < kb; j++, it++, s = s + 1 == ST ? (ph ^= 1, 0) : s + 1) {
+                if (!wait_bar(&sm.full[s], ph, abort)) {
+                    ok = false;
+                    break;
+                }
+                tc::tc_fence_after();
+                const uint64_t da = da0 + s * (a_bytes >> 4), db = db0 + s * (BN * kTileK >> 4);
+                if (tc::elect_one()) {
 #pragma unroll
                     for (int ks = 0; ks < kTileK / 32; ks++) tc::mma_i8(d, da + 2 * ks, db + 2 * ks, idesc, (j | ks) != 0);
                     tc::mma_commit(&sm.empty[s]);
+                    if (j + 1 == kb) tc::mma_commit(&sm.tfull[buf]);
                 }
-                if (ok) tc::mma_commit(&sm.tfull[buf]);
-            }
-            if (!ok || *abort) {   // no MMA may be running when TMEM is freed
-                for (uint32_t i = it > ST ? it - ST : 0; i < it; i++) drain_bar(&sm.empty[i % ST], (i / ST) & 1);
+                __syncwarp();
             }
         }
-        __syncwarp();
+        if (!ok || *abort) {   // no MMA may be running when TMEM is freed
+            for (uint32_t i = it > ST ? it - ST : 0; i < it; i++) drain_bar(&sm.empty[i % ST], (i / ST) & 1);
+            __syncwarp();
+        }
     } else {
         const int e = warp - 2, quad = warp & 3;
         constexpr int kBox = 128 / (int)sizeof(T);   // columns of one 128-byte box row
         uint32_t n = 0;
         int ob = 0;
+        tc::grid_wait();
         for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, n++) {
             uint32_t tm, tn;
             tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
@@ -336,7 +438,7 @@ k_w8a8_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             tc::tc_fence_after();
             const uint32_t src = tmem + buf * BN + ((uint32_t)(quad * 32) << 16);
             for (int c0 = 0; c0 < BN; c0 += kBox) {
-                if (n0 + c0 >= g.n) break;
+                if (n0 + c0 >= g.n || row0 >= g.m) break;
                 uint8_t* box = sm.out[e][ob];
                 // TMA clips a store to 16 bytes: a box that the row's end cuts elsewhere is stored by lanes
                 const bool by_tma = g.tma_out && (n0 + c0 + kBox <= g.n || g.n % (16 / sizeof(T)) == 0);
@@ -371,7 +473,7 @@ k_w8a8_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     tc::fence_async_shared();
                     __syncwarp();
                     if (lane == 0) {
-                        if (row0 < g.m) tc::tma_store_2d(&map_o, (int)(n0 + c0), (int)row0, box);
+                        tc::tma_store_2d(&map_o, (int)(n0 + c0), (int)row0, box);
                         tc::bulk_commit();
                     }
                     ob ^= 1;
