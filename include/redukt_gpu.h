@@ -343,6 +343,18 @@ uint64_t redukt_b200_w8a8_work_bytes(uint32_t n_tokens, uint32_t n_out, uint32_t
 /* Workspace with which redukt_b200_delta_chunk can cut requests (max_blocks of the block table). */
 uint64_t redukt_b200_delta_work_bytes(uint32_t max_blocks, uint32_t n_v_heads, uint32_t d_key, uint32_t d_value);
 
+/* One of the operators above with its arguments, in their order, as 64-bit words: pointers and integers as
+ * they are, the delta rule's scale as the bits of a double.  For hosts whose foreign calls convert every
+ * argument by itself: the conversions of delta_chunk's 30 arguments cost ctypes more than the launch.  A word
+ * that does not fit its argument is INVALID_ARGUMENT. */
+#define REDUKT_OP_PLAN_REQUESTS 0
+#define REDUKT_OP_DELTA_STEP 1
+#define REDUKT_OP_DELTA_CHUNK 2
+#define REDUKT_OP_QUANTIZE_TOKENS 3
+#define REDUKT_OP_W8A8_MATMUL 4
+#define REDUKT_OP_W8A8_LINEAR 5
+int32_t redukt_b200_ops_packed(uint32_t op, const uint64_t* words, uint32_t n_words);
+
 /* Last error message of this library (empty string when none). */
 const char* redukt_b200_last_error(void);
 

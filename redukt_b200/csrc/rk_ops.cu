@@ -7,7 +7,11 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstring>
 #include <mutex>
+#include <tuple>
+#include <type_traits>
+#include <utility>
 
 #include "../../include/redukt_gpu.h"
 #include "rk_delta.cuh"
@@ -326,6 +330,34 @@ int32_t matmul(const Device& d, const rk::w8::Args& a, int32_t out_dtype, cudaSt
 uint64_t quant_ld(uint32_t k) { return ceil_div(k, 16) * 16; }
 uint64_t quant_bytes(uint32_t n_tokens, uint32_t k) { return ceil_div((uint64_t)n_tokens * quant_ld(k), 256) * 256 + ceil_div(4ull * n_tokens, 256) * 256; }
 
+// Arguments of a call packed as 64-bit words, converted to an entry point's parameter types in order.
+template <class P>
+bool unpack(uint64_t w, P& out) {
+    if constexpr (std::is_pointer_v<P>) {
+        out = reinterpret_cast<P>(static_cast<uintptr_t>(w));
+        return true;
+    } else if constexpr (std::is_floating_point_v<P>) {
+        double d;
+        std::memcpy(&d, &w, sizeof d);
+        out = static_cast<P>(d);
+        return true;
+    } else {
+        out = static_cast<P>(w);
+        return static_cast<uint64_t>(static_cast<int64_t>(out)) == w || static_cast<uint64_t>(out) == w;
+    }
+}
+template <class... P, size_t... I>
+int32_t call_packed(int32_t (*fn)(P...), const uint64_t* words, uint32_t n_words, std::index_sequence<I...>) {
+    OP_REQUIRE(n_words == sizeof...(P), "ops_packed: %u words for %zu arguments", n_words, sizeof...(P));
+    std::tuple<P...> args;
+    OP_REQUIRE((unpack(words[I], std::get<I>(args)) && ...), "ops_packed: a word does not fit its argument");
+    return fn(std::get<I>(args)...);
+}
+template <class... P>
+int32_t call_packed(int32_t (*fn)(P...), const uint64_t* words, uint32_t n_words) {
+    return call_packed(fn, words, n_words, std::index_sequence_for<P...>{});
+}
+
 }  // namespace
 
 extern "C" {
@@ -477,6 +509,21 @@ int32_t redukt_b200_w8a8_linear(const void* d_x, int32_t dtype, uint32_t n_token
     if (int32_t rc = quantize(d_x, dtype, n_tokens, k, ld_x, q, quant_ld(k), s, st)) return rc;
     rk::w8::Args a = {q, s, d_w, d_w_scale, quant_ld(k), ld_w, ld_out, n_tokens, n_out, k, d_out};
     return matmul(*d, a, out_dtype, st, true);
+}
+
+int32_t redukt_b200_ops_packed(uint32_t op, const uint64_t* words, uint32_t n_words) {
+    OP_REQUIRE(words, "ops_packed: NULL argument");
+    switch (op) {
+        case REDUKT_OP_PLAN_REQUESTS: return call_packed(redukt_b200_plan_requests, words, n_words);
+        case REDUKT_OP_DELTA_STEP: return call_packed(redukt_b200_delta_step, words, n_words);
+        case REDUKT_OP_DELTA_CHUNK: return call_packed(redukt_b200_delta_chunk, words, n_words);
+        case REDUKT_OP_QUANTIZE_TOKENS: return call_packed(redukt_b200_quantize_tokens, words, n_words);
+        case REDUKT_OP_W8A8_MATMUL: return call_packed(redukt_b200_w8a8_matmul, words, n_words);
+        case REDUKT_OP_W8A8_LINEAR: return call_packed(redukt_b200_w8a8_linear, words, n_words);
+        default: break;
+    }
+    set_err("ops_packed: unknown operator %u", op);
+    return BACKEND_INVALID_ARGUMENT;
 }
 
 }  // extern "C"

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import enum
 import os
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -41,9 +42,16 @@ KERNEL_CLASSES = ("embed", "norm", "in_proj", "x_proj", "scan", "out_proj", "hea
 # operators over a ragged batch (absent from libraries built before them)
 OPS_SYMBOLS = ("redukt_b200_ops_error", "redukt_b200_plan_requests", "redukt_b200_delta_step", "redukt_b200_delta_chunk",
                "redukt_b200_delta_work_bytes", "redukt_b200_quantize_tokens", "redukt_b200_w8a8_matmul",
-               "redukt_b200_w8a8_linear", "redukt_b200_w8a8_work_bytes")
+               "redukt_b200_w8a8_linear", "redukt_b200_w8a8_work_bytes", "redukt_b200_ops_packed")
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+# records of redukt_b200_ops_packed: one 64-bit word per argument (Q pointers and unsigned, q signed, d the scale)
+_PLAN = struct.Struct("=2Qq Q4q 9Q")
+_STEP = struct.Struct("=3Qq2Q q2Q 4q 5q dq Q2q 2Q")
+_CHUNK = struct.Struct("=3Qq2Q 2q3Q 4q 5q dq Q2q Q2q 2Qq Q")
+_QUANT = struct.Struct("=Q4q Qq 2Q")
+_MATMUL = struct.Struct("=QqQq QqQ2q Q2q QqQ")
+_LINEAR = struct.Struct("=Q4q QqQq Q2q QqQ")
 
 
 class BackendResult(enum.IntEnum):
@@ -156,17 +164,9 @@ class PluginLibrary:
             L.redukt_b200_last_error.argtypes, L.redukt_b200_last_error.restype = [], ctypes.c_char_p
         self.has_ops = all(hasattr(L, s) for s in OPS_SYMBOLS)
         if self.has_ops:
-            vp, u64, f32 = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_float
-            heads, strides = [u32] * 4, [u64] * 5
+            u64 = ctypes.c_uint64
             L.redukt_b200_ops_error.argtypes = [u32p]
-            L.redukt_b200_plan_requests.argtypes = [vp, vp, u32, vp, u32, u32, u32, u32] + [vp] * 9
-            L.redukt_b200_delta_step.argtypes = ([vp, vp, vp, i32, vp, vp, u32, vp, vp] + heads + strides +
-                                                 [f32, i32, vp, u32, u64, vp, vp])
-            L.redukt_b200_delta_chunk.argtypes = ([vp, vp, vp, i32, vp, vp, u32, u32, vp, vp, vp] + heads + strides +
-                                                  [f32, i32, vp, u32, u64, vp, u32, u32, vp, vp, u64, vp])
-            L.redukt_b200_quantize_tokens.argtypes = [vp, i32, u32, u32, u64, vp, u64, vp, vp]
-            L.redukt_b200_w8a8_matmul.argtypes = [vp, u64, vp, u32, vp, u64, vp, u32, u32, vp, i32, u64, vp, u64, vp]
-            L.redukt_b200_w8a8_linear.argtypes = [vp, i32, u32, u32, u64, vp, u64, vp, u32, vp, i32, u64, vp, u64, vp]
+            L.redukt_b200_ops_packed.argtypes = [u32, ctypes.c_char_p, u32]
             for s in OPS_SYMBOLS:
                 getattr(L, s).restype = u64 if s.endswith("work_bytes") else i32
             L.redukt_b200_w8a8_work_bytes.argtypes = [u32, u32, u32]
@@ -222,23 +222,25 @@ class PluginLibrary:
             raise PluginError("redukt_b200_ops_error", code, self.last_error())
         return int(w[0])
 
+    def _packed(self, op: int, record: struct.Struct, *words) -> BackendResult:
+        code = self._ops().redukt_b200_ops_packed(op, record.pack(*words), record.size // 8)
+        return BackendResult.OK if code == 0 else BackendResult.from_code(code)
+
     def plan_requests(self, d_lengths: int, d_want: int, n: int, d_used: int, n_slots: int, block: int, max_tokens: int,
                       max_blocks: int, d_cu: int, d_slots: int, d_fresh: int, d_used_out: int, d_token_slot: int,
                       d_token_pos: int, d_block_base: int, d_blocks: int, stream: int = 0) -> BackendResult:
         """Token offsets, slots, token maps and block table of a ragged batch (redukt_b200_plan_requests)."""
-        return BackendResult.from_code(self._ops().redukt_b200_plan_requests(
-            d_lengths, d_want, n, d_used, n_slots, block, max_tokens, max_blocks, d_cu, d_slots, d_fresh, d_used_out,
-            d_token_slot, d_token_pos, d_block_base, d_blocks, stream or None))
+        return self._packed(0, _PLAN, d_lengths, d_want, n, d_used, n_slots, block, max_tokens, max_blocks, d_cu, d_slots,
+                            d_fresh, d_used_out, d_token_slot, d_token_pos, d_block_base, d_blocks, stream)
 
     def delta_step(self, d_q: int, d_k: int, d_v: int, dtype: int, d_log_decay: int, d_beta: int, n_streams: int,
                    d_slots: int, d_fresh: int, n_qk_heads: int, n_v_heads: int, d_key: int, d_value: int, ld_q: int,
                    ld_k: int, ld_v: int, ld_gate: int, ld_out: int, scale: float, l2norm: int, d_state: int, n_slots: int,
                    slot_stride: int, d_out: int, stream: int = 0) -> BackendResult:
         """The gated delta rule for one token of each stream (redukt_b200_delta_step)."""
-        return BackendResult.from_code(self._ops().redukt_b200_delta_step(
-            d_q, d_k, d_v, dtype, d_log_decay, d_beta, n_streams, d_slots, d_fresh or None, n_qk_heads, n_v_heads, d_key,
-            d_value, ld_q, ld_k, ld_v, ld_gate, ld_out, scale, l2norm, d_state, n_slots, slot_stride, d_out,
-            stream or None))
+        return self._packed(1, _STEP, d_q, d_k, d_v, dtype, d_log_decay, d_beta, n_streams, d_slots, d_fresh, n_qk_heads,
+                            n_v_heads, d_key, d_value, ld_q, ld_k, ld_v, ld_gate, ld_out, scale, l2norm, d_state, n_slots,
+                            slot_stride, d_out, stream)
 
     def delta_chunk(self, d_q: int, d_k: int, d_v: int, dtype: int, d_log_decay: int, d_beta: int, n_tokens: int,
                     n_requests: int, d_cu: int, d_slots: int, d_fresh: int, n_qk_heads: int, n_v_heads: int, d_key: int,
@@ -246,10 +248,10 @@ class PluginLibrary:
                     d_state: int, n_slots: int, slot_stride: int, d_blocks: int, block: int, max_blocks: int, d_out: int,
                     d_work: int = 0, work_bytes: int = 0, stream: int = 0) -> BackendResult:
         """The gated delta rule over every token of each request (redukt_b200_delta_chunk)."""
-        return BackendResult.from_code(self._ops().redukt_b200_delta_chunk(
-            d_q, d_k, d_v, dtype, d_log_decay, d_beta, n_tokens, n_requests, d_cu, d_slots, d_fresh or None, n_qk_heads,
-            n_v_heads, d_key, d_value, ld_q, ld_k, ld_v, ld_gate, ld_out, scale, l2norm, d_state, n_slots, slot_stride,
-            d_blocks or None, block, max_blocks, d_out, d_work or None, work_bytes, stream or None))
+        return self._packed(2, _CHUNK, d_q, d_k, d_v, dtype, d_log_decay, d_beta, n_tokens, n_requests, d_cu, d_slots,
+                            d_fresh, n_qk_heads, n_v_heads, d_key, d_value, ld_q, ld_k, ld_v, ld_gate, ld_out, scale,
+                            l2norm, d_state, n_slots, slot_stride, d_blocks, block, max_blocks, d_out, d_work, work_bytes,
+                            stream)
 
     def delta_work_bytes(self, max_blocks: int, n_v_heads: int, d_key: int, d_value: int) -> int:
         return int(self._ops().redukt_b200_delta_work_bytes(max_blocks, n_v_heads, d_key, d_value))
@@ -257,24 +259,21 @@ class PluginLibrary:
     def quantize_tokens(self, d_x: int, dtype: int, n_tokens: int, k: int, ld_x: int, d_q: int, ld_q: int, d_scale: int,
                         stream: int = 0) -> BackendResult:
         """Rows to int8 with one scale each (redukt_b200_quantize_tokens)."""
-        return BackendResult.from_code(self._ops().redukt_b200_quantize_tokens(d_x, dtype, n_tokens, k, ld_x, d_q, ld_q,
-                                                                               d_scale, stream or None))
+        return self._packed(3, _QUANT, d_x, dtype, n_tokens, k, ld_x, d_q, ld_q, d_scale, stream)
 
     def w8a8_matmul(self, d_a: int, ld_a: int, d_a_scale: int, n_tokens: int, d_w: int, ld_w: int, d_w_scale: int,
                     n_out: int, k: int, d_out: int, out_dtype: int, ld_out: int, d_work: int = 0, work_bytes: int = 0,
                     stream: int = 0) -> BackendResult:
         """int8 x int8 with a scale per token and channel (redukt_b200_w8a8_matmul)."""
-        return BackendResult.from_code(self._ops().redukt_b200_w8a8_matmul(
-            d_a, ld_a, d_a_scale, n_tokens, d_w, ld_w, d_w_scale, n_out, k, d_out, out_dtype, ld_out, d_work or None,
-            work_bytes, stream or None))
+        return self._packed(4, _MATMUL, d_a, ld_a, d_a_scale, n_tokens, d_w, ld_w, d_w_scale, n_out, k, d_out, out_dtype,
+                            ld_out, d_work, work_bytes, stream)
 
     def w8a8_linear(self, d_x: int, dtype: int, n_tokens: int, k: int, ld_x: int, d_w: int, ld_w: int, d_w_scale: int,
                     n_out: int, d_out: int, out_dtype: int, ld_out: int, d_work: int, work_bytes: int,
                     stream: int = 0) -> BackendResult:
         """Quantise each token, then multiply by int8 weights (redukt_b200_w8a8_linear)."""
-        return BackendResult.from_code(self._ops().redukt_b200_w8a8_linear(
-            d_x, dtype, n_tokens, k, ld_x, d_w, ld_w, d_w_scale, n_out, d_out, out_dtype, ld_out, d_work, work_bytes,
-            stream or None))
+        return self._packed(5, _LINEAR, d_x, dtype, n_tokens, k, ld_x, d_w, ld_w, d_w_scale, n_out, d_out, out_dtype,
+                            ld_out, d_work, work_bytes, stream)
 
     def w8a8_work_bytes(self, n_tokens: int, n_out: int, k: int) -> int:
         return int(self._ops().redukt_b200_w8a8_work_bytes(n_tokens, n_out, k))

@@ -1,0 +1,51 @@
+"""redukt_b200_ops_packed: the operators with their arguments as 64-bit words.  No compute calls."""
+import ctypes
+import struct
+
+import pytest
+
+from redukt_b200 import build as B
+from redukt_b200 import plugin as P
+from redukt_b200.plugin import BackendResult, PluginLibrary
+
+BAD = BackendResult.INVALID_ARGUMENT
+
+
+@pytest.fixture(scope="module")
+def lib():
+    B.build()
+    return PluginLibrary()
+
+
+def test_unknown_operator_and_missing_words(lib):
+    call = lib.lib.redukt_b200_ops_packed
+    words = struct.pack("=32Q", *range(32))
+    assert call(6, words, 32) == BAD and "unknown operator" in lib.last_error()
+    assert call(1, None, 25) == BAD
+    for op, record in enumerate((P._PLAN, P._STEP, P._CHUNK, P._QUANT, P._MATMUL, P._LINEAR)):
+        n = record.size // 8
+        for count in (0, n - 1, n + 1):
+            assert call(op, words, count) == BAD, (op, count)
+            assert "words for" in lib.last_error()
+
+
+@pytest.mark.parametrize("value", [-1, 1 << 32, (1 << 32) + 4, 1 << 62])
+def test_words_that_do_not_fit_a_32_bit_argument(lib, value):
+    """None of them may arrive as its low 32 bits."""
+    assert lib.quantize_tokens(256, 0, value, 64, 64, 256, 64, 256) == BAD
+    assert "does not fit" in lib.last_error()
+    assert lib.delta_step(256, 256, 256, 0, 256, 256, 0, 256, 0, 1, 1, value, 64, 64, 64, 64, 1, 64, 1.0, 0, 256, 1, 4096, 256) == BAD
+    assert "does not fit" in lib.last_error()
+
+
+def test_the_direct_symbols_answer_alike(lib):
+    """The C entry points themselves, through plain ctypes conversions."""
+    L, u32, u64, i32, vp, f32 = lib.lib, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_float
+    L.redukt_b200_quantize_tokens.argtypes = [vp, i32, u32, u32, u64, vp, u64, vp, vp]
+    assert L.redukt_b200_quantize_tokens(256, 0, 0, 64, 64, 256, 64, 256, None) == BackendResult.OK
+    assert L.redukt_b200_quantize_tokens(256, 0, 4, 64, 63, 256, 64, 256, None) == BAD
+    L.redukt_b200_delta_step.argtypes = [vp, vp, vp, i32, vp, vp, u32, vp, vp] + [u32] * 4 + [u64] * 5 + [f32, i32, vp, u32, u64, vp, vp]
+    args = [256, 256, 256, 0, 256, 256, 0, 256, None, 1, 1, 64, 64, 64, 64, 64, 1, 64, 1.0, 0, 256, 1, 4096, 256, None]
+    assert L.redukt_b200_delta_step(*args) == BackendResult.OK
+    args[11] = 65
+    assert L.redukt_b200_delta_step(*args) == BAD and "key size 65" in lib.last_error()
