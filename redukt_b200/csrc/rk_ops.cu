@@ -81,7 +81,7 @@ int32_t device(Device** out) {
         OP_CK(cudaGetSymbolAddress(&p, g_ops_err));
         d.err = static_cast<uint32_t*>(p);
         OP_CK(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
-        OP_CK(cudaFuncSetAttribute(rk::plan::k_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::plan::Smem)));
+        OP_CK(cudaFuncSetAttribute(rk::plan::k_plan<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::plan::Smem<1024>)));
         OP_CK(cudaFuncSetAttribute(rk::delta::k_delta_scan<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::delta::ScanSmem<64>)));
         OP_CK(cudaFuncSetAttribute(rk::delta::k_delta_scan<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::delta::ScanSmem<128>)));
         OP_CK((set_chunk_smem<64, float, false>()));
@@ -215,15 +215,32 @@ int32_t w8_check(const char* what, uint32_t n_tokens, uint32_t n_out, uint32_t k
     return BACKEND_OK;
 }
 
-int32_t quantize(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q, uint64_t ld_q,
-                 float* d_scale, cudaStream_t st) {
+template <class T, int kRowWarps>
+void launch_quant(const T* x, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* q, uint64_t ld_q, float* scale, cudaStream_t st) {
     using namespace rk::w8;
-    if (dtype == REDUKT_DTYPE_F32)
-        k_quant_tokens<float><<<n_tokens, kQuantThreads, 0, st>>>((const float*)d_x, k, ld_x, d_q, ld_q, d_scale);
-    else
-        k_quant_tokens<__nv_bfloat16><<<n_tokens, kQuantThreads, 0, st>>>((const __nv_bfloat16*)d_x, k, ld_x, d_q, ld_q, d_scale);
+    const unsigned rows = kQuantThreads / 32 / kRowWarps;
+    k_quant_tokens<T, kRowWarps><<<(unsigned)ceil_div(n_tokens, rows), kQuantThreads, 0, st>>>(x, n_tokens, k, ld_x, q, ld_q, scale);
+}
+
+// Warps per token: enough to hold the row in registers, and more while the batch leaves SMs without a block.
+template <class T>
+int32_t quantize_t(const Device& d, const T* x, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* q, uint64_t ld_q, float* scale,
+                   cudaStream_t st) {
+    const uint64_t vecs = ceil_div(k, 16 / sizeof(T));
+    int warps = 1;
+    while (warps < 8 && (vecs > 32ull * warps * rk::w8::kHold || (8ull / warps * d.sms > n_tokens && vecs > 32ull * warps))) warps *= 2;
+    if (warps == 1) launch_quant<T, 1>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
+    else if (warps == 2) launch_quant<T, 2>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
+    else if (warps == 4) launch_quant<T, 4>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
+    else launch_quant<T, 8>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
     OP_CK(cudaGetLastError());
     return BACKEND_OK;
+}
+
+int32_t quantize(const Device& d, const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q, uint64_t ld_q,
+                 float* d_scale, cudaStream_t st) {
+    return dtype == REDUKT_DTYPE_F32 ? quantize_t(d, (const float*)d_x, n_tokens, k, ld_x, d_q, ld_q, d_scale, st)
+                                     : quantize_t(d, (const __nv_bfloat16*)d_x, n_tokens, k, ld_x, d_q, ld_q, d_scale, st);
 }
 
 // A 2-D tensor map over rows of `width` elements, boxes of 128 bytes x box_rows in the 128-byte swizzle.
@@ -385,12 +402,17 @@ int32_t redukt_b200_plan_requests(const uint32_t* d_lengths, const uint32_t* d_w
     OP_REQUIRE(d_used != d_used_out || n_slots == 0, "plan_requests: used and used_out are the same buffer");
     Device* d = nullptr;
     if (int32_t rc = device(&d)) return rc;
-    rk::plan::Args a = {d_lengths, d_want, d_used, n, n_slots, block, max_tokens, max_blocks, d_cu, d_slots, d_fresh, d_used_out,
+    int shift = 0;
+    while (shift < 32 && (1ull << shift) < block) shift++;
+    if ((1ull << shift) != block) shift = -1;
+    rk::plan::Args a = {d_lengths, d_want, d_used, n, n_slots, block, max_tokens, max_blocks, shift, d_cu, d_slots, d_fresh, d_used_out,
                         d_token_slot, d_token_pos, d_block_base, d_blocks, d->err};
     // every block repeats the scans, so a block is worth adding only with a few thousand tokens to fill
-    const uint64_t fill = std::max<uint64_t>(ceil_div(max_tokens, 8192), ceil_div(max_blocks, 4096));
+    const bool small = n <= 1024 && n_slots <= 1024;
+    const uint64_t fill = std::max<uint64_t>(ceil_div(max_tokens, small ? 2048 : 8192), ceil_div(max_blocks, 4096));
     const unsigned grid = (unsigned)std::min<uint64_t>(std::max<uint64_t>(fill, 1), (uint64_t)d->sms);
-    rk::plan::k_plan<<<grid, rk::plan::kThreads, sizeof(rk::plan::Smem), stream_of(cuda_stream)>>>(a);
+    if (small) rk::plan::k_plan<256><<<grid, 256, sizeof(rk::plan::Smem<256>), stream_of(cuda_stream)>>>(a);
+    else rk::plan::k_plan<1024><<<grid, 1024, sizeof(rk::plan::Smem<1024>), stream_of(cuda_stream)>>>(a);
     OP_CK(cudaGetLastError());
     return BACKEND_OK;
 }
@@ -459,7 +481,9 @@ int32_t redukt_b200_quantize_tokens(const void* d_x, int32_t dtype, uint32_t n_t
     if (n_tokens == 0) return BACKEND_OK;
     OP_REQUIRE(d_x && d_q && d_scale, "quantize_tokens: NULL argument");
     OP_REQUIRE(aligned(d_x, dtype_size(dtype)) && aligned(d_scale, 4), "quantize_tokens: misaligned pointer");
-    return quantize(d_x, dtype, n_tokens, k, ld_x, d_q, ld_q, d_scale, stream_of(cuda_stream));
+    Device* d = nullptr;
+    if (int32_t rc = device(&d)) return rc;
+    return quantize(*d, d_x, dtype, n_tokens, k, ld_x, d_q, ld_q, d_scale, stream_of(cuda_stream));
 }
 
 uint64_t redukt_b200_delta_work_bytes(uint32_t max_blocks, uint32_t n_v_heads, uint32_t d_key, uint32_t d_value) {
@@ -506,7 +530,7 @@ int32_t redukt_b200_w8a8_linear(const void* d_x, int32_t dtype, uint32_t n_token
         return out_dtype == REDUKT_DTYPE_F32 ? few<__nv_bfloat16, float>(*d, a, (const __nv_bfloat16*)d_x, ld_x, st, false)
                                              : few<__nv_bfloat16, __nv_bfloat16>(*d, a, (const __nv_bfloat16*)d_x, ld_x, st, false);
     }
-    if (int32_t rc = quantize(d_x, dtype, n_tokens, k, ld_x, q, quant_ld(k), s, st)) return rc;
+    if (int32_t rc = quantize(*d, d_x, dtype, n_tokens, k, ld_x, q, quant_ld(k), s, st)) return rc;
     rk::w8::Args a = {q, s, d_w, d_w_scale, quant_ld(k), ld_w, ld_out, n_tokens, n_out, k, d_out};
     return matmul(*d, a, out_dtype, st, true);
 }

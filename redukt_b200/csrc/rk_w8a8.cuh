@@ -29,10 +29,10 @@ __device__ __forceinline__ int quant_one(float v, float inv) {
 
 __device__ __forceinline__ float row_scale(float amax) { return amax > 0.f ? __fmul_rn(amax, 1.f / 127.f) : 1.f; }
 
-// One block per token: the row's largest magnitude (exact in any order), then its 8-bit values.
+// kRowWarps warps per token: the row's largest magnitude (exact in any order), then its 8-bit values.
 // Bound by the bytes of the row in and out: it is read once, as 16-byte vectors kept in registers
 // (up to kHold a thread; longer or unaligned rows are read again).
-constexpr int kQuantThreads = 128;
+constexpr int kQuantThreads = 256;
 constexpr int kHold = 8;
 
 template <class T>
@@ -42,72 +42,92 @@ struct Vec {   // 16 bytes of activations
     __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(&raw)[i]); }
 };
 
+// quant_one for a finite inv, where |v inv| is at most 127.00002 (or NaN, which converts to 0): the largest
+// float below 1/2 added towards v's sign, then cut off, is round half away from zero (1/2 itself would take
+// the float below 1/2 up to 1); a third of the instructions of the general form.
+__device__ __forceinline__ int quant_fast(float v, float inv) {
+    const float t = __fmul_rn(v, inv);
+    return __float2int_rz(__fadd_rn(t, copysignf(0.49999997f, t)));
+}
+__device__ __forceinline__ uint32_t pack_s8(int a, int b, int c, int d) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 t;\n\tcvt.pack.sat.s8.s32.b32 t, %4, %3, 0;\n\tcvt.pack.sat.s8.s32.b32 %0, %2, %1, t;\n\t}"
+        : "=r"(r) : "r"(a), "r"(b), "r"(c), "r"(d));
+    return r;
+}
+
 template <class T>
 __device__ __forceinline__ void put_quant(int8_t* q, const Vec<T>& v, float inv) {   // 8 (bf16) or 4 (f32) bytes
     uint32_t w[Vec<T>::kN / 4];
 #pragma unroll
-    for (int i = 0; i < Vec<T>::kN; i++) {
-        const uint32_t b = (uint32_t)(quant_one(v.get(i), inv) & 255) << (8 * (i & 3));
-        w[i >> 2] = (i & 3) ? w[i >> 2] | b : b;
+    for (int i = 0; i < Vec<T>::kN / 4; i++) {
+        if (inv < __int_as_float(0x7f800000))
+            w[i] = pack_s8(quant_fast(v.get(4 * i), inv), quant_fast(v.get(4 * i + 1), inv), quant_fast(v.get(4 * i + 2), inv),
+                           quant_fast(v.get(4 * i + 3), inv));
+        else
+            w[i] = pack_s8(quant_one(v.get(4 * i), inv), quant_one(v.get(4 * i + 1), inv), quant_one(v.get(4 * i + 2), inv),
+                           quant_one(v.get(4 * i + 3), inv));
     }
     if constexpr (Vec<T>::kN == 8) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(q) = w[0];
 }
 
-__device__ __forceinline__ float block_max(float m, float* part) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
-    __syncthreads();
-    m = part[0];
-#pragma unroll
-    for (int i = 1; i < kQuantThreads / 32; i++) m = fmaxf(m, part[i]);
-    return m;
-}
-
-template <class T>
-__global__ void __launch_bounds__(kQuantThreads) k_quant_tokens(const T* __restrict__ x, uint32_t k, uint64_t ld_x, int8_t* __restrict__ q,
-                                                                uint64_t ld_q, float* __restrict__ scale) {
+template <class T, int kRowWarps>
+__global__ void __launch_bounds__(kQuantThreads) k_quant_tokens(const T* __restrict__ x, uint32_t rows, uint32_t k, uint64_t ld_x,
+                                                                int8_t* __restrict__ q, uint64_t ld_q, float* __restrict__ scale) {
     __shared__ float part[kQuantThreads / 32];
     tc::grid_trigger();   // a product launched after this kernel sets itself up meanwhile
     constexpr int N = Vec<T>::kN;
-    const T* xr = x + blockIdx.x * ld_x;
-    int8_t* qr = q + blockIdx.x * ld_q;
+    constexpr uint32_t kRowThreads = 32 * kRowWarps, kRows = kQuantThreads / kRowThreads;
+    const uint32_t tid = threadIdx.x % kRowThreads;
+    const uint64_t row = (uint64_t)blockIdx.x * kRows + threadIdx.x / kRowThreads;
+    const bool live = row < rows;   // no early return: the rows of a block share its barrier
+    const T* xr = x + (live ? row : 0) * ld_x;
+    int8_t* qr = q + (live ? row : 0) * ld_q;
     const bool wide = ((reinterpret_cast<uintptr_t>(xr) & 15) | (reinterpret_cast<uintptr_t>(qr) & (N - 1))) == 0;
-    const uint32_t nv = wide ? k / N : 0;   // whole vectors; the rest one by one
+    const uint32_t kk = live ? k : 0u, nv = wide ? kk / N : 0u;   // whole vectors; the rest one by one
     float m = 0.f;
     Vec<T> v[kHold];
 #pragma unroll
     for (int i = 0; i < kHold; i++) {
-        const uint32_t j = threadIdx.x + i * kQuantThreads;
-        if (j < nv) {
-            v[i].raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
-#pragma unroll
-            for (int c = 0; c < N; c++) m = fmaxf(m, fabsf(v[i].get(c)));
-        }
+        const uint32_t j = tid + i * kRowThreads;
+        if (j < nv) v[i].raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
+        else v[i].raw = make_uint4(0, 0, 0, 0);
     }
-    for (uint32_t j = threadIdx.x + kHold * kQuantThreads; j < nv; j += kQuantThreads) {
+#pragma unroll
+    for (int i = 0; i < kHold; i++)
+#pragma unroll
+        for (int c = 0; c < N; c++) m = fmaxf(m, fabsf(v[i].get(c)));
+    for (uint32_t j = tid + kHold * kRowThreads; j < nv; j += kRowThreads) {
         Vec<T> u;
         u.raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
 #pragma unroll
         for (int c = 0; c < N; c++) m = fmaxf(m, fabsf(u.get(c)));
     }
-    for (uint32_t c = nv * N + threadIdx.x; c < k; c += kQuantThreads) m = fmaxf(m, fabsf(to_f32(xr[c])));
-    m = block_max(m, part);
+    for (uint32_t c = nv * N + tid; c < kk; c += kRowThreads) m = fmaxf(m, fabsf(to_f32(xr[c])));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    if (kRowWarps > 1) {
+        const uint32_t warp = threadIdx.x >> 5, w0 = warp / kRowWarps * kRowWarps;
+        if ((threadIdx.x & 31) == 0) part[warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kRowWarps; i++) m = fmaxf(m, part[w0 + i]);
+    }
     const float s = row_scale(m);
     const float inv = __fdiv_rn(1.f, s);
 #pragma unroll
     for (int i = 0; i < kHold; i++) {
-        const uint32_t j = threadIdx.x + i * kQuantThreads;
+        const uint32_t j = tid + i * kRowThreads;
         if (j < nv) put_quant(qr + (uint64_t)j * N, v[i], inv);
     }
-    for (uint32_t j = threadIdx.x + kHold * kQuantThreads; j < nv; j += kQuantThreads) {
+    for (uint32_t j = tid + kHold * kRowThreads; j < nv; j += kRowThreads) {
         Vec<T> u;
         u.raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
         put_quant(qr + (uint64_t)j * N, u, inv);
     }
-    for (uint32_t c = nv * N + threadIdx.x; c < k; c += kQuantThreads) qr[c] = (int8_t)quant_one(to_f32(xr[c]), inv);
-    if (threadIdx.x == 0) scale[blockIdx.x] = s;
+    for (uint32_t c = nv * N + tid; c < kk; c += kRowThreads) qr[c] = (int8_t)quant_one(to_f32(xr[c]), inv);
+    if (live && tid == 0) scale[row] = s;
 }
 
 struct Args {
