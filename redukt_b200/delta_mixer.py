@@ -1,0 +1,172 @@
+"""A token-mixing layer on the ragged-batch operators: plan, int8 projections, gated delta rule.
+
+An example of how the operators are used together over a pool of state slots:
+
+    mixer = DeltaMixer(PluginLibrary(), d_model=768, n_heads=12, d_key=64, n_slots=64)
+    y, slots = mixer.prefill(x, lengths)     # whole windows, ragged: one row of x per token
+    y = mixer.step(x_next, slots)            # then one token of each stream
+
+prefill plans the batch from the windows' lengths on the GPU (plan_requests), projects all tokens
+to q, k, v and the gates with one int8 product (w8a8_linear), runs the gated delta rule over every
+window from its slot (delta_chunk, reading q, k and v in place from the projection's rows) and
+projects back; step does the same for single tokens with delta_step.  Weights are seeded.
+
+`python -m redukt_b200.delta_mixer` compares windows prefilled whole with windows prefilled in part and
+stepped to their end, and prints the time of both.  Needs torch (for device memory) and a B200.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from .plugin import DTYPE_F32, BackendResult, PluginError, PluginLibrary
+
+NEW = -1   # UINT32_MAX: a request that starts a new stream
+
+
+class DeltaMixer:
+    def __init__(self, library: PluginLibrary, d_model: int, n_heads: int, d_key: int, n_slots: int,
+                 d_value: Optional[int] = None, n_v_heads: Optional[int] = None, block: int = 256, seed: int = 0):
+        self.lib = library
+        self.d_model, self.hk, self.dk = d_model, n_heads, d_key
+        self.hv, self.dv = n_v_heads or n_heads, d_value or d_key
+        self.n_slots, self.block = n_slots, block
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        # rows of the fused projection: q, k, v, decay gate, write gate
+        self.n_in = 2 * self.hk * self.dk + self.hv * self.dv + 2 * self.hv
+        self.w_in, self.s_in = self._weights(self.n_in, d_model, gen)
+        self.w_out, self.s_out = self._weights(d_model, self.hv * self.dv, gen)
+        # decay rates 1..16 over the heads; step bias = softplus^-1 of log-uniform [1e-3, 1e-1]
+        self.rate = torch.linspace(1.0, 16.0, self.hv, device="cuda")
+        dt = torch.exp(math.log(1e-3) + torch.rand(self.hv, generator=gen, device="cuda") * math.log(100.0))
+        self.dt_bias = torch.log(torch.expm1(dt))
+        self.state = torch.zeros(n_slots, self.hv, self.dv, self.dk, device="cuda")
+        self.used = torch.zeros(n_slots, dtype=torch.uint8, device="cuda")
+
+    @staticmethod
+    def _weights(rows: int, cols: int, gen) -> Tuple[torch.Tensor, torch.Tensor]:
+        """N(0, 1 / cols) as int8 with one scale per row; rows padded to 16 bytes."""
+        w = torch.randn(rows, cols, generator=gen, device="cuda") / math.sqrt(cols)
+        scale = w.abs().amax(1) / 127.0
+        q = torch.zeros(rows, -(-cols // 16) * 16, dtype=torch.int8, device="cuda")
+        q[:, :cols] = torch.round(w / scale[:, None]).to(torch.int8)
+        return q, scale
+
+    def _check(self, what: str, code: BackendResult) -> None:
+        if code != BackendResult.OK:
+            raise PluginError(what, code, self.lib.last_error())
+
+    def _linear(self, x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+        m, k, n = x.shape[0], x.shape[1], w.shape[0]
+        out = torch.empty(m, n, device="cuda")
+        work = torch.empty(max(256, self.lib.w8a8_work_bytes(m, n, k)), dtype=torch.uint8, device="cuda")
+        self._check("w8a8_linear", self.lib.w8a8_linear(
+            x.data_ptr(), DTYPE_F32, m, k, x.stride(0), w.data_ptr(), w.stride(0), scale.data_ptr(), n, out.data_ptr(),
+            DTYPE_F32, n, work.data_ptr(), work.numel(), torch.cuda.current_stream().cuda_stream))
+        return out
+
+    def _project(self, x: torch.Tensor):
+        """(rows of q | k | v, log decay, write gate) of each token."""
+        p = self._linear(x, self.w_in, self.s_in)
+        gates = p[:, self.n_in - 2 * self.hv:]
+        g = -self.rate * torch.nn.functional.softplus(gates[:, :self.hv] + self.dt_bias)
+        return p, g.contiguous(), torch.sigmoid(gates[:, self.hv:]).contiguous()
+
+    def _rule(self, p: torch.Tensor):
+        """The arguments that both forms of the rule share: q, k, v in place in the projection's rows."""
+        at = p.data_ptr()
+        q, k, v = at, at + 4 * self.hk * self.dk, at + 8 * self.hk * self.dk
+        out = torch.empty(p.shape[0], self.hv * self.dv, device="cuda")
+        ld = p.stride(0)
+        tail = (self.hk, self.hv, self.dk, self.dv, ld, ld, ld, self.hv, out.stride(0), 1.0 / math.sqrt(self.dk), 1,
+                self.state.data_ptr(), self.n_slots, self.state.stride(0))
+        return (q, k, v, DTYPE_F32), tail, out
+
+    def plan(self, lengths: torch.Tensor, want: Optional[torch.Tensor], tokens: int) -> dict:
+        """plan_requests of a batch: lengths and want [n] int32 on the GPU; marks the slots that it gives."""
+        n = lengths.numel()
+        blocks = tokens // self.block + n
+        want = torch.full((n,), NEW, dtype=torch.int32, device="cuda") if want is None else want
+
+        def i32(*shape):
+            return torch.empty(*shape, dtype=torch.int32, device="cuda")
+
+        p = dict(cu=i32(n + 1), slot=i32(n), fresh=i32(n), used=torch.empty_like(self.used), token_slot=i32(tokens),
+                 token_pos=i32(tokens), base=i32(n + 1), blocks=i32(blocks, 2), n=n, n_blocks=blocks)
+        self._check("plan_requests", self.lib.plan_requests(
+            lengths.data_ptr(), want.data_ptr(), n, self.used.data_ptr(), self.n_slots, self.block, tokens, blocks,
+            p["cu"].data_ptr(), p["slot"].data_ptr(), p["fresh"].data_ptr(), p["used"].data_ptr(),
+            p["token_slot"].data_ptr(), p["token_pos"].data_ptr(), p["base"].data_ptr(), p["blocks"].data_ptr(),
+            torch.cuda.current_stream().cuda_stream))
+        self.used = p["used"]
+        return p
+
+    def prefill(self, x: torch.Tensor, lengths: torch.Tensor, want: Optional[torch.Tensor] = None):
+        """x [tokens, d_model] f32, the windows one after the other -> (outputs, each window's slot)."""
+        plan = self.plan(lengths, want, x.shape[0])
+        p, g, beta = self._project(x)
+        head, tail, out = self._rule(p)
+        work = torch.empty(self.lib.delta_work_bytes(plan["n_blocks"], self.hv, self.dk, self.dv), dtype=torch.uint8, device="cuda")
+        self._check("delta_chunk", self.lib.delta_chunk(
+            *head, g.data_ptr(), beta.data_ptr(), x.shape[0], plan["n"], plan["cu"].data_ptr(), plan["slot"].data_ptr(),
+            plan["fresh"].data_ptr(), *tail, plan["blocks"].data_ptr(), self.block, plan["n_blocks"], out.data_ptr(),
+            work.data_ptr(), work.numel(), torch.cuda.current_stream().cuda_stream))
+        return self._linear(out, self.w_out, self.s_out), plan["slot"]
+
+    def step(self, x: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+        """x [streams, d_model] f32, one token of each of the slots' streams -> outputs."""
+        p, g, beta = self._project(x)
+        head, tail, out = self._rule(p)
+        self._check("delta_step", self.lib.delta_step(
+            *head, g.data_ptr(), beta.data_ptr(), x.shape[0], slots.data_ptr(), 0, *tail, out.data_ptr(),
+            torch.cuda.current_stream().cuda_stream))
+        return self._linear(out, self.w_out, self.s_out)
+
+
+def run(lengths: Sequence[int] = (300, 1, 77, 512, 64), steps: int = 40, d_model: int = 768, n_heads: int = 12,
+        d_key: int = 64, seed: int = 0) -> dict:
+    """Windows of lengths[i] + steps tokens, once prefilled whole, once prefilled to lengths[i] and stepped to the end."""
+    lib = PluginLibrary()
+    n = len(lengths)
+    gen = torch.Generator(device="cuda").manual_seed(seed + 1)
+    windows = [torch.randn(t + steps, d_model, generator=gen, device="cuda") for t in lengths]
+
+    def batch(parts):
+        return torch.cat(parts), torch.tensor([len(p) for p in parts], dtype=torch.int32, device="cuda")
+
+    def timed(fn):
+        torch.cuda.synchronize()
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        got = fn()
+        b.record()
+        torch.cuda.synchronize()
+        return got, a.elapsed_time(b)
+
+    whole = DeltaMixer(lib, d_model, n_heads, d_key, n_slots=n + 3, seed=seed)
+    x, sizes = batch(windows)
+    whole.prefill(x, sizes)                       # warm-up
+    whole.used.zero_()
+    (y, slots), prefill_ms = timed(lambda: whole.prefill(x, sizes))
+
+    part = DeltaMixer(lib, d_model, n_heads, d_key, n_slots=n + 3, seed=seed)
+    x0, sizes0 = batch([w[:t] for w, t in zip(windows, lengths)])
+    _, slots0 = part.prefill(x0, sizes0)
+    rows = torch.stack([w[-steps:] for w in windows], 1)          # [steps, n, d_model]
+    outs, step_ms = timed(lambda: [part.step(rows[t], slots0) for t in range(steps)])
+    ends = torch.cumsum(sizes.long(), 0)
+    tails = torch.stack([y[e - steps:e] for e in ends.tolist()], 1)
+    got = torch.stack(outs)
+    word = lib.ops_error()
+    state, ref = part.state[slots0.long()], whole.state[slots.long()]
+    return dict(tokens=int(x.shape[0]), streams=n, prefill_ms=prefill_ms, step_ms=step_ms / steps, error_word=word,
+                state_off=float((state - ref).norm() / ref.norm()), out_off=float((got - tails).norm() / tails.norm()))
+
+
+if __name__ == "__main__":
+    r = run()
+    print("prefill of %d tokens: %.3f ms; a step of %d streams: %.3f ms" % (r["tokens"], r["prefill_ms"], r["streams"], r["step_ms"]))
+    print("stepped against prefilled: state %.1e, outputs %.1e (relative 2-norms), error word %d" %
+          (r["state_off"], r["out_off"], r["error_word"]))

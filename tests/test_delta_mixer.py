@@ -1,0 +1,78 @@
+"""The example layer: plan, int8 projections, chunked and per-token rule together.
+
+Tolerances: the projections of a token have the same bits in prefill and step, so the states differ by the
+rule's two forms only: 2e-5 each way of the 64-bit answer, 4e-5 together.  The output projection quantises
+values that differ by that much: where one lies that near to a rounding boundary its int8 value moves by
+one, 1 / 127 of the row's largest value and of the order of 3 / 127 of the row's rms; with a share p of
+the values doing so the output moves by sqrt(p) times that.  Values spread over about 60 steps rms, so p is
+about 2 * 4e-5 * 60 = 5e-3, and sqrt(5e-3) * 3 / 127 = 1.7e-3: OUT = 2e-3."""
+import numpy as np
+import pytest
+
+STATE, OUT = 4e-5, 2e-3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,steps,n_heads,d_key", [((300, 1, 77, 512, 64), 20, 12, 64), ((33,), 5, 3, 128), ((2000, 3), 3, 2, 128)])
+def test_prefill_and_steps_agree(lengths, steps, n_heads, d_key):
+    from redukt_b200.delta_mixer import run
+    r = run(lengths, steps, d_model=256, n_heads=n_heads, d_key=d_key)
+    assert r["error_word"] == 0
+    assert r["state_off"] <= STATE and r["out_off"] <= OUT, r
+
+
+@pytest.mark.gpu
+def test_continued_streams_keep_their_slots():
+    """Two prefills of the same streams, the second in another order, against one of the joined windows."""
+    import torch
+
+    from redukt_b200.delta_mixer import NEW, DeltaMixer
+    from redukt_b200.plugin import PluginLibrary
+    lib = PluginLibrary()
+    x = torch.randn(3, 90, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+
+    def i32(*v):
+        return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+    a = DeltaMixer(lib, 128, 2, 64, n_slots=6, seed=1)
+    _, one = a.prefill(x.reshape(-1, 128), i32(90, 90, 90))
+    b = DeltaMixer(lib, 128, 2, 64, n_slots=6, seed=1)
+    _, first = b.prefill(x[:, :40].reshape(-1, 128), i32(40, 40, 40))
+    assert first.tolist() == [0, 1, 2] and b.used.tolist() == [1, 1, 1, 0, 0, 0]
+    order = [2, 0, 1]
+    rest = torch.cat([x[i, 40:] for i in order] + [x[0, :7]])          # and a new stream beside them
+    _, second = b.prefill(rest, i32(50, 50, 50, 7), torch.cat([first[order], i32(NEW)]))
+    assert second.tolist() == [2, 0, 1, 3] and b.used.tolist() == [1, 1, 1, 1, 0, 0]
+    assert lib.ops_error() == 0
+    for i in range(3):
+        ref, got = a.state[one[i].long()], b.state[first[i].long()]
+        assert float((got - ref).norm() / ref.norm()) <= STATE
+
+
+@pytest.mark.gpu
+def test_layer_against_64_bits():
+    """The whole layer from its definition: numpy, 64 bits but for the int8 values, which are defined in 32."""
+    import torch
+
+    from redukt_b200.delta_mixer import DeltaMixer
+    from redukt_b200.plugin import PluginLibrary
+    from test_ops_delta import rule
+    from test_ops_w8a8 import product, quantize
+    mixer = DeltaMixer(PluginLibrary(), 128, 2, 64, n_slots=4, n_v_heads=4, seed=5)
+    x = torch.randn(150, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(6))
+    y, slots = mixer.prefill(x, torch.tensor([150], dtype=torch.int32, device="cuda"))
+
+    def linear(rows, w, s):
+        q, sc = quantize(rows)
+        return product(q, sc, w.cpu().numpy()[:, :rows.shape[1]], s.cpu().numpy())
+
+    p = linear(x.cpu().numpy(), mixer.w_in, mixer.s_in).astype(np.float64)
+    hk, hv, dk, dv = mixer.hk, mixer.hv, mixer.dk, mixer.dv
+    q, k, v, a, b = np.split(p, np.cumsum([hk * dk, hk * dk, hv * dv, hv]), axis=1)
+    g = -mixer.rate.double().cpu().numpy() * np.log1p(np.exp(a + mixer.dt_bias.double().cpu().numpy()))
+    o, S = rule(q.reshape(-1, hk, dk), k.reshape(-1, hk, dk), v.reshape(-1, hv, dv), g, 1 / (1 + np.exp(-b)),
+                np.zeros((hv, dv, dk)), 1 / np.sqrt(dk), True)
+    got = mixer.state[slots.long()[0]].cpu().numpy()
+    assert np.linalg.norm(got - S) / np.linalg.norm(S) <= STATE
+    want = linear(o.reshape(150, -1).astype(np.float32), mixer.w_out, mixer.s_out)
+    assert np.linalg.norm(y.cpu().numpy() - want) / np.linalg.norm(want) <= OUT
