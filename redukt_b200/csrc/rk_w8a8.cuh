@@ -266,8 +266,7 @@ constexpr int kTcThreads = 192;
 constexpr long long kWaitCycles = 4000000000ll;   // about 2 s
 
 // Stages: as many as fit beside the rest.  A batch of fewer than 128 tokens stages only its rows (the product
-// still reads 128 rows: the next stages' bytes, whose sums nobody reads), so more weights are in flight;
-// 16 x 8,192 x 8,192 with 64-channel tiles is bound by that.
+// still reads 128 rows: the next stages' bytes, whose sums nobody reads).
 constexpr int kMaxStages = 20;
 constexpr size_t kSmemMax = 232448;
 
