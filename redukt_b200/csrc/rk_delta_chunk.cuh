@@ -98,12 +98,11 @@ __device__ __forceinline__ uint64_t segment_id(const ChunkArgs& c, uint64_t firs
     return first_row / ((uint64_t)c.block * c.merge) + req + seg_index;
 }
 
-// 2^(14 - e) for a largest magnitude in [2^e, 2^(e+1)), and its inverse; finite for every m.
+// 2^(14 - e) for a largest magnitude m in [2^e, 2^(e+1)), and its inverse; finite for every m (0 included).
 __device__ __forceinline__ float row_pow(float m, float& inv) {
-    const int e = (int)(__float_as_uint(m) >> 23);
-    const int s = min(268 - e, 253);
-    inv = m > 0.f ? __uint_as_float((uint32_t)(254 - s) << 23) : 1.f;
-    return m > 0.f ? __uint_as_float((uint32_t)s << 23) : 1.f;
+    const int s = min(268 - (int)(__float_as_uint(m) >> 23), 253);
+    inv = __uint_as_float((uint32_t)(254 - s) << 23);
+    return __uint_as_float((uint32_t)s << 23);
 }
 // max that keeps a NaN out of the scale; the NaN itself stays in the value
 __device__ __forceinline__ float amax(float m, float x) { return fmaxf(m, fabsf(x)); }
@@ -127,6 +126,15 @@ __device__ __forceinline__ float2 mul2(float2 x, float2 a) {
     return r;
 }
 
+__device__ __forceinline__ void scale2(float* y, const float* x, float s) {
+    const float2 r = mul2(make_float2(x[0], x[1]), make_float2(s, s));
+    y[0] = r.x, y[1] = r.y;
+}
+__device__ __forceinline__ void add2(float* y, const float* x, float2 s) {   // y += x s
+    const float2 r = fma2(make_float2(x[0], x[1]), s, make_float2(y[0], y[1]));
+    y[0] = r.x, y[1] = r.y;
+}
+
 // two values, times s, as one register of each plane
 __device__ __forceinline__ uint32_t pack_hi(float x, float y, float s) {
     const float2 v = mul2(make_float2(x, y), make_float2(s, s));
@@ -146,6 +154,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the first product of a sum: d = a b
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const __half* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -529,12 +543,15 @@ struct Block {
         const __half* at = strips + strip_base(ib) + ((lane & 7) + (lane >> 4) * 8) * strip_ld(ib) + 16 * jb + ((lane >> 3) & 1) * 8;
         ldsm4(lo, at + 16 * strip_ld(ib));
         ldsm4(hi, at);
-#pragma unroll
-        for (int c = 0; c < 4; c++) d0[c] = d1[c] = 0.f;
     }
     __device__ __forceinline__ void round(int r, const uint32_t (&ah)[4], const uint32_t (&al)[4]) {
-        mma_f16(d0, r == 1 ? al : ah, r == 0 ? lo[0] : hi[0], r == 0 ? lo[1] : hi[1]);
-        mma_f16(d1, r == 1 ? al : ah, r == 0 ? lo[2] : hi[2], r == 0 ? lo[3] : hi[3]);
+        if (r == 0) {
+            mma_f16_first(d0, ah, lo[0], lo[1]);
+            mma_f16_first(d1, ah, lo[2], lo[3]);
+            return;
+        }
+        mma_f16(d0, r == 1 ? al : ah, hi[0], hi[1]);
+        mma_f16(d1, r == 1 ? al : ah, hi[2], hi[3]);
     }
 };
 
@@ -556,10 +573,6 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
             V[n][c] = (i < len && !ident) ? vp[(at + i) * a.ld_v + (c >> 1) * 8] : T(0.f);
         }
     float X[kC / 8][4], O[kC / 8][4];
-#pragma unroll
-    for (int n = 0; n < kC / 8; n++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) X[n][c] = O[n][c] = 0.f;
     {
         float m[2][4] = {};   // several chains of maxima, joined at the end
 #pragma unroll
@@ -586,11 +599,15 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
             }
 #pragma unroll
             for (int nn = 0; nn < kNB; nn++) {
-                mma_f16(X[2 * nn], lo, bk[nn][0], bk[nn][1]);
-                mma_f16(X[2 * nn + 1], lo, bk[nn][2], bk[nn][3]);
+                const auto first = [&](float(&d)[4], uint32_t b0, uint32_t b1) {
+                    if (ks == 0) mma_f16_first(d, lo, b0, b1);
+                    else mma_f16(d, lo, b0, b1);
+                };
+                first(X[2 * nn], bk[nn][0], bk[nn][1]);
+                first(X[2 * nn + 1], bk[nn][2], bk[nn][3]);
                 if (kOut) {
-                    mma_f16(O[2 * nn], lo, bq[nn][0], bq[nn][1]);
-                    mma_f16(O[2 * nn + 1], lo, bq[nn][2], bq[nn][3]);
+                    first(O[2 * nn], bq[nn][0], bq[nn][1]);
+                    first(O[2 * nn + 1], bq[nn][2], bq[nn][3]);
                 }
             }
             if (KP == 2) {
@@ -622,14 +639,22 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
         }
         // right-hand side R = b (V - e^c X), and the state's part of the output
 #pragma unroll
-        for (int n = 0; n < kC / 8; n++)
+        for (int n = 0; n < kC / 8; n++) {
+            const int i = 8 * n + 2 * t;
+            const float2 be = *reinterpret_cast<const float2*>(&sm.beta[i]), ak = *reinterpret_cast<const float2*>(&sm.ak[i]);
+            const float2 cq = kOut ? *reinterpret_cast<const float2*>(&sm.cq[i]) : make_float2(0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int i = 8 * n + 2 * t + (c & 1);
-                const float sv = c < 2 ? sv0 : sv1;
-                X[n][c] = sm.beta[i] * (to_f32(V[n][c]) - sm.ak[i] * (sv * X[n][c]));
-                if (kOut) O[n][c] = sm.cq[i] * (sv * O[n][c]);
+            for (int c = 0; c < 4; c += 2) {
+                const float sv = c ? sv1 : sv0;
+                const float2 y = mul2(make_float2(X[n][c], X[n][c + 1]), make_float2(-sv, -sv));
+                const float2 r = mul2(be, fma2(ak, y, make_float2(to_f32(V[n][c]), to_f32(V[n][c + 1]))));
+                X[n][c] = r.x, X[n][c + 1] = r.y;
+                if (kOut) {
+                    const float2 o = mul2(cq, mul2(make_float2(O[n][c], O[n][c + 1]), make_float2(sv, sv)));
+                    O[n][c] = o.x, O[n][c + 1] = o.y;
+                }
             }
+        }
     }
     // U in the place of R; O_i += P_ij U_j
     static_assert(kNB == 2, "two blocks of 16 tokens");
@@ -650,18 +675,21 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
         for (int i = 0; i < kNB; i++) {
             const float db = sm.dscale[i];
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                X[2 * i][c] = d[i].d0[c] * (db * inv[i][c >> 1]);
-                X[2 * i + 1][c] = d[i].d1[c] * (db * inv[i][c >> 1]);
+            for (int c = 0; c < 4; c += 2) {
+                const float f = db * inv[i][c >> 1];
+                scale2(X[2 * i] + c, d[i].d0 + c, f);
+                scale2(X[2 * i + 1] + c, d[i].d1 + c, f);
             }
         }
     }
     const auto add_out = [&](const Block& p, int i, int j, const float (&us)[2]) {
-        const float* ps = &sm.pscale[j][16 * i + 2 * t];
+        const float2 ps = *reinterpret_cast<const float2*>(&sm.pscale[j][16 * i + 2 * t]);
+        const float2 qs = *reinterpret_cast<const float2*>(&sm.pscale[j][16 * i + 2 * t + 8]);
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            O[2 * i][c] = fmaf(ps[c & 1] * us[c >> 1], p.d0[c], O[2 * i][c]);
-            O[2 * i + 1][c] = fmaf(ps[8 + (c & 1)] * us[c >> 1], p.d1[c], O[2 * i + 1][c]);
+        for (int c = 0; c < 4; c += 2) {
+            const float2 u = make_float2(us[c >> 1], us[c >> 1]);
+            add2(O[2 * i] + c, p.d0 + c, mul2(ps, u));
+            add2(O[2 * i + 1] + c, p.d1 + c, mul2(qs, u));
         }
     };
     {
@@ -677,9 +705,10 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
         }
         const float b = -sm.bscale;
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            X[2][c] = fmaf(b * us[c >> 1], b10.d0[c], X[2][c]);
-            X[3][c] = fmaf(b * us[c >> 1], b10.d1[c], X[3][c]);
+        for (int c = 0; c < 4; c += 2) {
+            const float2 f = make_float2(b * us[c >> 1], b * us[c >> 1]);
+            add2(X[2] + c, b10.d0 + c, f);
+            add2(X[3] + c, b10.d1 + c, f);
         }
         if (kOut) {
             add_out(p00, 0, 0, us);
@@ -702,17 +731,16 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
             }
     }
     // S = e^{c_32} S + sum_j (w_j u_j) k_j^T
-    float n0 = 0.f, n1 = 0.f;
+    float w0[2] = {}, w1[2] = {};
 #pragma unroll
-    for (int n = 0; n < kC / 8; n++)
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const float w = sm.wk[8 * n + 2 * t + c];
-            X[n][c] *= w;
-            X[n][2 + c] *= w;
-            n0 = amax(n0, X[n][c]);
-            n1 = amax(n1, X[n][2 + c]);
-        }
+    for (int n = 0; n < kC / 8; n++) {
+        const float2 w = *reinterpret_cast<const float2*>(&sm.wk[8 * n + 2 * t]);
+        const float2 x = mul2(make_float2(X[n][0], X[n][1]), w), y = mul2(make_float2(X[n][2], X[n][3]), w);
+        X[n][0] = x.x, X[n][1] = x.y, X[n][2] = y.x, X[n][3] = y.y;
+        w0[n & 1] = amax(amax(w0[n & 1], x.x), x.y);
+        w1[n & 1] = amax(amax(w1[n & 1], y.x), y.y);
+    }
+    const float n0 = fmaxf(w0[0], w0[1]), n1 = fmaxf(w1[0], w1[1]);
     float iv0, iv1;
     const float q0 = row_pow(quad_max(n0), iv0), q1 = row_pow(quad_max(n1), iv1);
 #pragma unroll
@@ -726,7 +754,7 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
     const int trow = (lane & 7) + ((lane >> 3) & 1) * 8, tcol = (lane >> 4) * 8;
 #pragma unroll
     for (int n0 = 0; n0 < NT / 2; n0 += 2) {   // 32 state columns at a time, four accumulators a round
-        float d[4][4] = {};
+        float d[4][4];
         uint32_t b[kNB][2][4];
 #pragma unroll
         for (int jb = 0; jb < kNB; jb++)
@@ -736,8 +764,13 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
         for (int jb = 0; jb < kNB; jb++)
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                mma_f16(d[2 * u], ul[jb], b[jb][u][0], b[jb][u][1]);
-                mma_f16(d[2 * u + 1], ul[jb], b[jb][u][2], b[jb][u][3]);
+                if (jb == 0) {
+                    mma_f16_first(d[2 * u], ul[jb], b[jb][u][0], b[jb][u][1]);
+                    mma_f16_first(d[2 * u + 1], ul[jb], b[jb][u][2], b[jb][u][3]);
+                } else {
+                    mma_f16(d[2 * u], ul[jb], b[jb][u][0], b[jb][u][1]);
+                    mma_f16(d[2 * u + 1], ul[jb], b[jb][u][2], b[jb][u][3]);
+                }
             }
         if (KP == 2) {
 #pragma unroll
