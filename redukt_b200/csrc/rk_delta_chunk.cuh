@@ -74,9 +74,14 @@ struct alignas(16) Chunk {
     float dscale[kNB], bscale;          // scales of D and B
 };
 
+// Row of a warp's 16 staged values; the odd 16 bytes keep 8 rows of the mma layout out of each other's banks.
+template <class T>
+constexpr int kVLd = 16 + 16 / (int)sizeof(T);
+
 template <int DK, class T, bool kWide>
 struct alignas(16) ChunkSmem {
     Chunk<DK, T> c[kWide ? 2 : 1];
+    T v[ChunkCfg<DK, T, kWide>::kRows / 16][2][kC * kVLd<T>];   // each stepping warp's values of this and the next chunk
     uint4 raw[kPrep * 4 * (DK * (int)sizeof(T) / 128)];   // the next chunk's k and q, each thread's own vectors
 };
 
@@ -280,22 +285,18 @@ __device__ __forceinline__ void prep_sync() { asm volatile("bar.sync 1, %0;" ::"
 // four 16-byte parts swapped so that the mma layout's stores meet two to a bank at most.
 __device__ __forceinline__ int wait_at(int row, int col) { return col * 16 + ((((row >> 2) ^ (col >> 1)) & 3) << 2) + (row & 3); }
 
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-
 // What the four preparing warps bring from one chunk to the next.
 template <int DK, class T, bool kOut>
 struct Source {
     const T* p;             // this thread's first row: k's for warps 0 and 1, q's for 2 and 3
     uint64_t ld;
     const float *g, *beta;  // of token `lane`
-    const T* v;             // token threadIdx.x / 4 of the chunk: the block's value rows
-    uint64_t ld_g, ld_v;
+    uint64_t ld_g;
     float gate, b;          // the staged chunk's
     int warp, row, l;       // row of the 8-lane group in the chunk, lane in it
     bool wide;
-    uint32_t v_bytes;
 
-    __device__ __forceinline__ void init(const Args& a, uint64_t t0, uint32_t h, uint32_t hq, uint32_t v_row, uint32_t v_rows) {
+    __device__ __forceinline__ void init(const Args& a, uint64_t t0, uint32_t h, uint32_t hq) {
         const int lane = threadIdx.x & 31;
         warp = threadIdx.x >> 5;
         row = (warp & 1) * 16 + (lane >> 3);
@@ -306,9 +307,6 @@ struct Source {
         g = a.g + (t0 + lane) * a.ld_g + h;
         beta = a.beta + (t0 + lane) * a.ld_g + h;
         ld_g = a.ld_g;
-        ld_v = a.ld_v;
-        v = (const T*)a.v + (t0 + (threadIdx.x >> 2)) * ld_v + (uint64_t)h * a.dv + v_row;
-        v_bytes = v_row < a.dv ? min(v_rows, a.dv - v_row) * (uint32_t)sizeof(T) : 0u;
     }
     // Starts the copies of the next chunk of `len` tokens; rows past its end repeat the last one.
     __device__ __forceinline__ void stage(uint4* raw, int len) {
@@ -319,7 +317,6 @@ struct Source {
                 const int r = min(row + 4 * i, len - 1) - row;
                 RowLoad<DK, T>::stage(slot + i * RowLoad<DK, T>::NV * kPrep, p + (int64_t)r * (int64_t)ld, wide, l);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
             p += kC * ld;
         }
         const bool live = (int)(threadIdx.x & 31) < len;
@@ -327,9 +324,6 @@ struct Source {
         b = live && warp == 1 ? *beta : 0.f;
         g += kC * ld_g;
         beta += kC * ld_g;
-        if ((int)(threadIdx.x >> 2) < len)   // the values, read straight from global memory, on their way to L2
-            for (uint32_t o = (threadIdx.x & 3) * 128; o < v_bytes; o += 512) prefetch_l2((const char*)v + o);
-        v += kC * ld_v;
     }
 };
 
@@ -365,9 +359,9 @@ __device__ __forceinline__ void prepare_chunk(Chunk<DK, T>& sm, const uint4* raw
     } else {
         sm.beta[lane] = src.b;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");   // this thread's own copies
     if (kOut || key) {
         RowLoad<DK, T> rows[4];
-        asm volatile("cp.async.wait_all;" ::: "memory");   // this thread's own copies
 #pragma unroll
         for (int i = 0; i < 4; i++) rows[i].unstage(raw + threadIdx.x + i * RowLoad<DK, T>::NV * kPrep);
         put_rows<DK, T>(rows, key ? sm.k[0] : sm.q[0], key ? sm.k[KP - 1] : sm.q[KP - 1], LD, key ? sm.sk : sm.sq, row, len, a.l2norm, l);
@@ -555,23 +549,35 @@ struct Block {
     }
 };
 
+// Starts the copies of a warp's 16 values of each of a chunk's `len` tokens (lane = token; past the end the last
+// token's, whose write gate is zero).
+template <class T>
+__device__ __forceinline__ void stage_values(T* dst, const T* src, uint64_t ld, int len, bool wide) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const int lane = threadIdx.x & 31;
+    const T* p = src + (uint64_t)min(lane, len - 1) * ld;
+    T* q = dst + lane * kVLd<T>;
+#pragma unroll
+    for (int c = 0; c < 16; c += N) {
+        if (wide) {
+            copy16(q + c, p + c);
+        } else {   // any alignment
+#pragma unroll
+            for (int i = 0; i < N; i++) q[c + i] = p[c + i];
+        }
+    }
+}
+
 // One chunk's step of 16 state rows, by one warp: S (rows row0 + g and + 8, columns 8 n + 2 t, + 1) to the
-// state after it, with outputs where kOut.  vp and op: v and out at (row 0, this thread's first state row).
+// state after it, with outputs where kOut.  vt: the warp's staged values at (token 0, this thread's first state
+// row); op: out at (row 0, that state row).
 template <int DK, class T, bool kOut>
-__device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)[DK / 8][4], const Args& a, const T* vp, T* op,
+__device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)[DK / 8][4], const Args& a, const T* vt, T* op,
                                               uint64_t at, int len, bool ident) {
     using Cfg = ChunkCfg<DK, T, false>;
     constexpr int LD = Cfg::LD, KP = Cfg::KP, NT = DK / 8;
     const int lane = threadIdx.x & 31, t = lane & 3;
-    // X = S K^T and O = S Q^T over the chunk; V meanwhile
-    T V[kC / 8][4];
-#pragma unroll
-    for (int n = 0; n < kC / 8; n++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const int i = 8 * n + 2 * t + (c & 1);
-            V[n][c] = (i < len && !ident) ? vp[(at + i) * a.ld_v + (c >> 1) * 8] : T(0.f);
-        }
+    // X = S K^T and O = S Q^T over the chunk
     float X[kC / 8][4], O[kC / 8][4];
     {
         float m[2][4] = {};   // several chains of maxima, joined at the end
@@ -647,7 +653,9 @@ __device__ __forceinline__ void consume_chunk(const Chunk<DK, T>& sm, float (&S)
             for (int c = 0; c < 4; c += 2) {
                 const float sv = c ? sv1 : sv0;
                 const float2 y = mul2(make_float2(X[n][c], X[n][c + 1]), make_float2(-sv, -sv));
-                const float2 r = mul2(be, fma2(ak, y, make_float2(to_f32(V[n][c]), to_f32(V[n][c + 1]))));
+                const T* v = vt + i * kVLd<T> + 4 * c;   // c = 2: eight rows on
+                const float2 vv = ident ? make_float2(0.f, 0.f) : make_float2(to_f32(v[0]), to_f32(v[kVLd<T>]));
+                const float2 r = mul2(be, fma2(ak, y, vv));
                 X[n][c] = r.x, X[n][c + 1] = r.y;
                 if (kOut) {
                     const float2 o = mul2(cq, mul2(make_float2(O[n][c], O[n][c + 1]), make_float2(sv, sv)));
@@ -868,14 +876,16 @@ __global__ void __launch_bounds__(ChunkCfg<DK, T, kWide>::kThreads, ChunkCfg<DK,
         }
         S[n][0] = x.x, S[n][1] = x.y, S[n][2] = y.x, S[n][3] = y.y;
     }
-    const T* vp = (const T*)a.v + (uint64_t)h * a.dv + row0 + g;
     T* op = (T*)a.out + (uint64_t)h * a.dv + row0 + g;
 
+    const T* vp = (const T*)a.v + (uint64_t)h * a.dv + row0;
+    const bool v_wide = ((reinterpret_cast<uintptr_t>(vp) | (a.ld_v * sizeof(T))) & 15) == 0, values = active && !ident;
+    T(*vt)[kC * kVLd<T>] = sm.v[kWide ? (warp < 4 ? 0 : warp - 4) : warp];
     const auto chunk_len = [&](uint64_t at) { return (int)min((uint64_t)kC, t1 - at); };
     if constexpr (kWide) {
         if (warp < 4) {
             Source<DK, T, kOut> in;
-            in.init(a, t0, h, hq, blockIdx.x * Cfg::kRows, Cfg::kRows);
+            in.init(a, t0, h, hq);
             if (t0 < t1) in.stage(sm.raw, chunk_len(t0));
             for (uint64_t at = t0, n = 0; at < t1; at += kC, n++) {
                 prepare_chunk<DK, T, kOut>(sm.c[n & 1], sm.raw, a, in, chunk_len(at));
@@ -884,19 +894,29 @@ __global__ void __launch_bounds__(ChunkCfg<DK, T, kWide>::kThreads, ChunkCfg<DK,
             }
             return;
         }
+        if (values && t0 < t1) stage_values(vt[0], vp + t0 * a.ld_v, a.ld_v, chunk_len(t0), v_wide);
         for (uint64_t at = t0, n = 0; at < t1; at += kC, n++) {
+            asm volatile("cp.async.wait_all;" ::: "memory");   // this chunk's values, staged a chunk ago
             __syncthreads();
-            if (active) consume_chunk<DK, T, kOut>(sm.c[n & 1], S, a, vp, op, at, chunk_len(at), ident);
+            if (values && at + kC < t1) stage_values(vt[(n & 1) ^ 1], vp + (at + kC) * a.ld_v, a.ld_v, chunk_len(at + kC), v_wide);
+            if (active) consume_chunk<DK, T, kOut>(sm.c[n & 1], S, a, vt[n & 1] + g, op, at, chunk_len(at), ident);
         }
     } else {
         Source<DK, T, kOut> in;
-        in.init(a, t0, h, hq, blockIdx.x * Cfg::kRows, Cfg::kRows);
-        if (t0 < t1) in.stage(sm.raw, chunk_len(t0));
-        for (uint64_t at = t0; at < t1; at += kC) {
-            prepare_chunk<DK, T, kOut>(sm.c[0], sm.raw, a, in, chunk_len(at));
-            if (at + kC < t1) in.stage(sm.raw, chunk_len(at + kC));
+        in.init(a, t0, h, hq);
+        if (t0 < t1) {
+            in.stage(sm.raw, chunk_len(t0));
+            if (values) stage_values(vt[0], vp + t0 * a.ld_v, a.ld_v, chunk_len(t0), v_wide);
+        }
+        int vb = 0;
+        for (uint64_t at = t0; at < t1; at += kC, vb ^= 1) {
+            prepare_chunk<DK, T, kOut>(sm.c[0], sm.raw, a, in, chunk_len(at));   // waits for the thread's copies, values too
+            if (at + kC < t1) {
+                in.stage(sm.raw, chunk_len(at + kC));
+                if (values) stage_values(vt[vb ^ 1], vp + (at + kC) * a.ld_v, a.ld_v, chunk_len(at + kC), v_wide);
+            }
             __syncthreads();
-            if (active) consume_chunk<DK, T, kOut>(sm.c[0], S, a, vp, op, at, chunk_len(at), ident);
+            if (active) consume_chunk<DK, T, kOut>(sm.c[0], S, a, vt[vb] + g, op, at, chunk_len(at), ident);
             __syncthreads();   // the shared operands are free again
         }
     }
@@ -915,11 +935,11 @@ __global__ void __launch_bounds__(ChunkCfg<DK, T, kWide>::kThreads, ChunkCfg<DK,
     }
 }
 
-// Start states of a request's segments: S, S M_0 + b_0, ...  grid (ceil(dv / 8), hv, requests), DK threads:
-// thread j owns column j of 8 state rows.  The chain is one small product per segment; every M and b is
+// Start states of a request's segments: S, S M_0 + b_0, ...  grid (ceil(dv / 8), hv, requests), 2 DK threads:
+// thread (half, j) owns column j of four of the block's 8 state rows.  The chain is one small product per segment; every M and b is
 // there beforehand, so they are copied to shared memory kScanAhead segments early and a step costs its
 // 8 DK^2 products and not the way to L2.
-constexpr int kScanRows = 8;
+constexpr int kScanRows = 8, kMine = kScanRows / 2;
 __host__ __device__ constexpr int scan_ahead(int dk) { return dk == 128 ? 2 : 4; }
 template <int DK>
 struct alignas(16) ScanSmem {
@@ -929,24 +949,25 @@ struct alignas(16) ScanSmem {
 };
 
 template <int DK>
-__global__ void __launch_bounds__(DK) k_delta_scan(ChunkArgs ca) {
+__global__ void __launch_bounds__(2 * DK) k_delta_scan(ChunkArgs ca) {
     extern __shared__ uint8_t raw[];
     ScanSmem<DK>& sm = *reinterpret_cast<ScanSmem<DK>*>(raw);
     constexpr int kAhead = scan_ahead(DK), kBufs = kAhead + 1;
     const Args& a = ca.a;
-    const uint32_t h = blockIdx.y, req = blockIdx.z, slot = a.slots[req], j = threadIdx.x, r0 = blockIdx.x * kScanRows;
+    const uint32_t h = blockIdx.y, req = blockIdx.z, slot = a.slots[req], j = threadIdx.x % DK, lr = threadIdx.x / DK * kMine,
+                   r0 = blockIdx.x * kScanRows;
     const uint64_t t0 = min(a.cu[req], a.n_rows), t1 = min(a.cu[req + 1], a.n_rows), seg = (uint64_t)ca.block * ca.merge;
     if (slot >= a.n_slots || t0 >= t1) {   // a fresh request without tokens still leaves a zero state
         if (slot < a.n_slots && a.fresh && a.fresh[req])
-            for (int r = 0; r < kScanRows; r++) a.state[slot * a.slot_stride + ((uint64_t)h * a.dv + r0 + r) * DK + j] = 0.f;
+            for (int r = 0; r < kMine; r++) a.state[slot * a.slot_stride + ((uint64_t)h * a.dv + r0 + lr + r) * DK + j] = 0.f;
         return;
     }
     const uint64_t per_head = (uint64_t)a.dv * DK;
     const bool zero = a.fresh && a.fresh[req];
-    float s[kScanRows];
+    float s[kMine];
 #pragma unroll
-    for (int r = 0; r < kScanRows; r++)
-        s[r] = zero ? 0.f : a.state[slot * a.slot_stride + h * per_head + (uint64_t)(r0 + r) * DK + j];
+    for (int r = 0; r < kMine; r++)
+        s[r] = zero ? 0.f : a.state[slot * a.slot_stride + h * per_head + (uint64_t)(r0 + lr + r) * DK + j];
     const uint32_t n_seg = (uint32_t)((t1 - t0 + seg - 1) / seg);
     const uint64_t first = segment_id(ca, t0, req, 0);
     const auto fetch = [&](uint32_t p) {   // segment p's M and b, one group of copies (empty past the last)
@@ -954,8 +975,8 @@ __global__ void __launch_bounds__(DK) k_delta_scan(ChunkArgs ca) {
             const uint64_t id = (first + p) * a.hv + h;
             const float* m = ca.m_seg + id * (DK * DK);
             const float* b = ca.b_seg + id * per_head + (uint64_t)r0 * DK;
-            for (int i = j * 4; i < DK * DK; i += DK * 4) copy16(&sm.m[p % kBufs][i], m + i);
-            for (int i = j * 4; i < kScanRows * DK; i += DK * 4) copy16(&sm.b[p % kBufs][i], b + i);
+            for (int i = threadIdx.x * 4; i < DK * DK; i += DK * 8) copy16(&sm.m[p % kBufs][i], m + i);
+            for (int i = threadIdx.x * 4; i < kScanRows * DK; i += DK * 8) copy16(&sm.b[p % kBufs][i], b + i);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -963,28 +984,28 @@ __global__ void __launch_bounds__(DK) k_delta_scan(ChunkArgs ca) {
     for (uint32_t p = 0; p < n_seg; p++) {
         const uint64_t id = (first + p) * a.hv + h;
 #pragma unroll
-        for (int r = 0; r < kScanRows; r++) ca.s_in[id * per_head + (uint64_t)(r0 + r) * DK + j] = s[r];
+        for (int r = 0; r < kMine; r++) ca.s_in[id * per_head + (uint64_t)(r0 + lr + r) * DK + j] = s[r];
         if (p + 1 == n_seg) break;
         fetch(p + kAhead);
 #pragma unroll
-        for (int r = 0; r < kScanRows; r++) reinterpret_cast<float*>(sm.rows[r])[j] = s[r];
+        for (int r = 0; r < kMine; r++) reinterpret_cast<float*>(sm.rows[lr + r])[j] = s[r];
         asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
         __syncthreads();
         const float* m = sm.m[p % kBufs] + j;
-        float d[kScanRows];
+        float d[kMine];
 #pragma unroll
-        for (int r = 0; r < kScanRows; r++) d[r] = 0.f;
+        for (int r = 0; r < kMine; r++) d[r] = 0.f;
 #pragma unroll 4
         for (int k = 0; k < DK / 4; k++) {
             const float m0 = m[(4 * k) * DK], m1 = m[(4 * k + 1) * DK], m2 = m[(4 * k + 2) * DK], m3 = m[(4 * k + 3) * DK];
 #pragma unroll
-            for (int r = 0; r < kScanRows; r++) {
-                const float4 x = sm.rows[r][k];
+            for (int r = 0; r < kMine; r++) {
+                const float4 x = sm.rows[lr + r][k];
                 d[r] = fmaf(x.x, m0, fmaf(x.y, m1, fmaf(x.z, m2, fmaf(x.w, m3, d[r]))));
             }
         }
 #pragma unroll
-        for (int r = 0; r < kScanRows; r++) s[r] = d[r] + sm.b[p % kBufs][r * DK + j];
+        for (int r = 0; r < kMine; r++) s[r] = d[r] + sm.b[p % kBufs][(lr + r) * DK + j];
         __syncthreads();   // rows and this buffer are free again
     }
     asm volatile("cp.async.wait_all;" ::: "memory");

@@ -185,7 +185,7 @@ int32_t launch_chunk(const Device& d, rk::delta::ChunkArgs ca, uint32_t max_bloc
         ca.s_in = ca.b_seg + segs * ca.a.hv * ca.a.dv * DK;
         ca.m_seg = ca.s_in + segs * ca.a.hv * ca.a.dv * DK;
         k_delta_chunk<DK, T, kWide, 1><<<dim3((unsigned)ceil_div(ca.a.dv + DK, Cfg::kRows), ca.a.hv, max_blocks), Cfg::kThreads, smem, st>>>(ca);
-        k_delta_scan<DK><<<dim3((unsigned)ceil_div(ca.a.dv, kScanRows), ca.a.hv, ca.a.n), DK, sizeof(ScanSmem<DK>), st>>>(ca);
+        k_delta_scan<DK><<<dim3((unsigned)ceil_div(ca.a.dv, kScanRows), ca.a.hv, ca.a.n), 2 * DK, sizeof(ScanSmem<DK>), st>>>(ca);
         k_delta_chunk<DK, T, kWide, 2><<<dim3(slices, ca.a.hv, max_blocks), Cfg::kThreads, smem, st>>>(ca);
     }
     OP_CK(cudaGetLastError());
