@@ -1,10 +1,12 @@
-// The gated delta rule over state slots: one token per stream (k_delta_step) and, token by token,
-// whole requests (k_delta_serial).
+// The gated delta rule over state slots, one token of each stream (whole requests: rk_delta_chunk.cuh).
 //
 // Per value head, S in R^{dv x dk} (a slot's state, f32, row-major), a_t = exp(g_t):
 //   u_t = b_t (v_t - a_t S_{t-1} k_t),  S_t = a_t S_{t-1} + u_t k_t^T,  o_t = scale S_t q_t
 // The output needs no second pass over the state: S_t q = a_t S_{t-1} q + u_t (k.q), so both row
-// products S_{t-1} k and S_{t-1} q come from one read of S_{t-1}.
+// products S_{t-1} k and S_{t-1} q come from one read of S_{t-1}.  What bounds it is that read and the
+// write of S_t: 256 streams x 16 heads of 128 x 128 move 540 MB in 83 us, 6.5 TB/s.  Eight lanes share a
+// row, so a row's loads are 128 contiguous bytes each and a product is summed in three shuffles; a warp
+// has eight rows in flight.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -14,14 +16,13 @@
 namespace rk {
 namespace delta {
 
-constexpr uint32_t kNone = 0xFFFFFFFFu;
 constexpr float kNormEps = 1e-6f;
 
 struct Args {
     const void *q, *k, *v;
     const float *g, *beta;
-    const uint32_t *cu, *slots, *fresh;   // cu: prefill only; fresh may be NULL (no stream starts from zero)
-    uint32_t n, n_rows;                   // requests or streams; rows of q/k/v
+    const uint32_t *cu, *slots, *fresh;   // cu: requests only; fresh may be NULL (no stream starts from zero)
+    uint32_t n, n_rows;                   // requests or streams; rows of q, k, v
     uint32_t hk, hv, dv;
     uint64_t ld_q, ld_k, ld_v, ld_g, ld_o;
     float scale;
@@ -148,32 +149,6 @@ __global__ void __launch_bounds__(kWarps * 32) k_delta_step(Args a) {
     const uint32_t hq = h / (a.hv / a.hk);
     R.token(a, (const T*)a.q + b * a.ld_q + (uint64_t)hq * DK, (const T*)a.k + b * a.ld_k + (uint64_t)hq * DK,
             (const T*)a.v + b * a.ld_v + (uint64_t)h * a.dv, o, a.g[b * a.ld_g + h], a.beta[b * a.ld_g + h], row0, grp, l);
-    R.store(st, row0, a.dv, grp, l);
-}
-
-// Every token of each request, one after the other, the state rows in registers.
-template <int DK, class T>
-__global__ void __launch_bounds__(kWarps * 32) k_delta_serial(Args a) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane >> 3, l = lane & 7;
-    const int row0 = (blockIdx.x * kWarps + warp) * 4 * kPass;
-    const uint32_t h = blockIdx.y, req = blockIdx.z, hq = h / (a.hv / a.hk);
-    const uint32_t slot = a.slots[req];
-    const uint64_t t0 = min(a.cu[req], a.n_rows), t1 = min(a.cu[req + 1], a.n_rows);
-    if (slot >= a.n_slots) {
-        const uint32_t r0 = blockIdx.x * kRows, w = min(a.dv, r0 + kRows) - r0;
-        for (uint64_t t = t0; t < t1; t++)
-            for (uint32_t r = threadIdx.x; r < w; r += blockDim.x)
-                put((T*)a.out + t * a.ld_o + (uint64_t)h * a.dv + r0 + r, 0.f);
-        if (t1 > t0 && h == 0 && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err, 1u);
-        return;
-    }
-    float* st = a.state + slot * a.slot_stride + (uint64_t)h * a.dv * DK;
-    Rows<DK, T> R;
-    R.load(st, row0, a.dv, grp, l, a.fresh && a.fresh[req]);
-    for (uint64_t t = t0; t < t1; t++)
-        R.token(a, (const T*)a.q + t * a.ld_q + (uint64_t)hq * DK, (const T*)a.k + t * a.ld_k + (uint64_t)hq * DK,
-                (const T*)a.v + t * a.ld_v + (uint64_t)h * a.dv, (T*)a.out + t * a.ld_o + (uint64_t)h * a.dv,
-                a.g[t * a.ld_g + h], a.beta[t * a.ld_g + h], row0, grp, l);
     R.store(st, row0, a.dv, grp, l);
 }
 

@@ -244,10 +244,10 @@ struct RowLoad {
     }
 };
 
-// 1 / sqrt(x): the hardware's estimate and one Newton step.
+// 1 / sqrt(x): the hardware's estimate and one Newton step (0 for an infinite x).
 __device__ __forceinline__ float inv_sqrt(float x) {
     const float y = rsqrtf(x);
-    return y * fmaf(-0.5f * x * y, y, 1.5f);
+    return y > 0.f ? y * fmaf(-0.5f * x * y, y, 1.5f) : y;
 }
 
 // Four rows of each 8-lane group: row, row + 4, row + 8, row + 12.

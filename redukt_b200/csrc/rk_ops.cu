@@ -215,32 +215,40 @@ int32_t w8_check(const char* what, uint32_t n_tokens, uint32_t n_out, uint32_t k
     return BACKEND_OK;
 }
 
-template <class T, int kRowWarps>
+template <class T, int kRowWarps, bool kWide>
 void launch_quant(const T* x, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* q, uint64_t ld_q, float* scale, cudaStream_t st) {
     using namespace rk::w8;
     const unsigned rows = kQuantThreads / 32 / kRowWarps;
-    k_quant_tokens<T, kRowWarps><<<(unsigned)ceil_div(n_tokens, rows), kQuantThreads, 0, st>>>(x, n_tokens, k, ld_x, q, ld_q, scale);
+    k_quant_tokens<T, kRowWarps, kWide><<<(unsigned)ceil_div(n_tokens, rows), kQuantThreads, 0, st>>>(x, n_tokens, k, ld_x, q, ld_q, scale);
 }
 
 // Warps per token: enough to hold the row in registers, and more while the batch leaves SMs without a block.
-template <class T>
+template <class T, bool kWide>
 int32_t quantize_t(const Device& d, const T* x, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* q, uint64_t ld_q, float* scale,
                    cudaStream_t st) {
-    const uint64_t vecs = ceil_div(k, 16 / sizeof(T));
+    const uint64_t items = kWide ? ceil_div(k, 16 / sizeof(T)) : k, hold = kWide ? rk::w8::kHold : rk::w8::kHoldSingle;
     int warps = 1;
-    while (warps < 8 && (vecs > 32ull * warps * rk::w8::kHold || (8ull / warps * d.sms > n_tokens && vecs > 32ull * warps))) warps *= 2;
-    if (warps == 1) launch_quant<T, 1>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
-    else if (warps == 2) launch_quant<T, 2>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
-    else if (warps == 4) launch_quant<T, 4>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
-    else launch_quant<T, 8>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
+    while (warps < 8 && (items > 32ull * warps * hold || (8ull / warps * d.sms > n_tokens && items > 32ull * warps))) warps *= 2;
+    if (warps == 1) launch_quant<T, 1, kWide>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
+    else if (warps == 2) launch_quant<T, 2, kWide>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
+    else if (warps == 4) launch_quant<T, 4, kWide>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
+    else launch_quant<T, 8, kWide>(x, n_tokens, k, ld_x, q, ld_q, scale, st);
     OP_CK(cudaGetLastError());
     return BACKEND_OK;
 }
 
+template <class T>
+int32_t quantize_rows(const Device& d, const T* x, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* q, uint64_t ld_q, float* scale,
+                      cudaStream_t st) {
+    const bool wide = aligned(x, 16) && ld_x * sizeof(T) % 16 == 0 && aligned(q, 8) && ld_q % 8 == 0;
+    return wide ? quantize_t<T, true>(d, x, n_tokens, k, ld_x, q, ld_q, scale, st)
+                : quantize_t<T, false>(d, x, n_tokens, k, ld_x, q, ld_q, scale, st);
+}
+
 int32_t quantize(const Device& d, const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q, uint64_t ld_q,
                  float* d_scale, cudaStream_t st) {
-    return dtype == REDUKT_DTYPE_F32 ? quantize_t(d, (const float*)d_x, n_tokens, k, ld_x, d_q, ld_q, d_scale, st)
-                                     : quantize_t(d, (const __nv_bfloat16*)d_x, n_tokens, k, ld_x, d_q, ld_q, d_scale, st);
+    return dtype == REDUKT_DTYPE_F32 ? quantize_rows(d, (const float*)d_x, n_tokens, k, ld_x, d_q, ld_q, d_scale, st)
+                                     : quantize_rows(d, (const __nv_bfloat16*)d_x, n_tokens, k, ld_x, d_q, ld_q, d_scale, st);
 }
 
 // A 2-D tensor map over rows of `width` elements, boxes of 128 bytes x box_rows in the 128-byte swizzle.

@@ -30,10 +30,11 @@ __device__ __forceinline__ int quant_one(float v, float inv) {
 __device__ __forceinline__ float row_scale(float amax) { return amax > 0.f ? __fmul_rn(amax, 1.f / 127.f) : 1.f; }
 
 // kRowWarps warps per token: the row's largest magnitude (exact in any order), then its 8-bit values.
-// Bound by the bytes of the row in and out: it is read once, as 16-byte vectors kept in registers
-// (up to kHold a thread; longer or unaligned rows are read again).
+// Bound by the bytes of the row in and out: it is read once and kept in registers, as 16-byte vectors where
+// every row starts on 16 bytes (kWide), else as single values by consecutive lanes; what a row has beyond
+// kHold vectors (kHoldSingle values) a thread is read again.
 constexpr int kQuantThreads = 256;
-constexpr int kHold = 8;
+constexpr int kHold = 8, kHoldSingle = 16;
 
 template <class T>
 struct Vec {   // 16 bytes of activations
@@ -49,6 +50,9 @@ __device__ __forceinline__ int quant_fast(float v, float inv) {
     const float t = __fmul_rn(v, inv);
     return __float2int_rz(__fadd_rn(t, copysignf(0.49999997f, t)));
 }
+__device__ __forceinline__ int quant_any(float v, float inv) {
+    return inv < __int_as_float(0x7f800000) ? quant_fast(v, inv) : quant_one(v, inv);
+}
 __device__ __forceinline__ uint32_t pack_s8(int a, int b, int c, int d) {
     uint32_t r;
     asm("{\n\t.reg .b32 t;\n\tcvt.pack.sat.s8.s32.b32 t, %4, %3, 0;\n\tcvt.pack.sat.s8.s32.b32 %0, %2, %1, t;\n\t}"
@@ -61,50 +65,58 @@ __device__ __forceinline__ void put_quant(int8_t* q, const Vec<T>& v, float inv)
     uint32_t w[Vec<T>::kN / 4];
 #pragma unroll
     for (int i = 0; i < Vec<T>::kN / 4; i++) {
-        if (inv < __int_as_float(0x7f800000))
-            w[i] = pack_s8(quant_fast(v.get(4 * i), inv), quant_fast(v.get(4 * i + 1), inv), quant_fast(v.get(4 * i + 2), inv),
-                           quant_fast(v.get(4 * i + 3), inv));
-        else
-            w[i] = pack_s8(quant_one(v.get(4 * i), inv), quant_one(v.get(4 * i + 1), inv), quant_one(v.get(4 * i + 2), inv),
-                           quant_one(v.get(4 * i + 3), inv));
+        w[i] = pack_s8(quant_any(v.get(4 * i), inv), quant_any(v.get(4 * i + 1), inv), quant_any(v.get(4 * i + 2), inv),
+                       quant_any(v.get(4 * i + 3), inv));
     }
     if constexpr (Vec<T>::kN == 8) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(q) = w[0];
 }
 
-template <class T, int kRowWarps>
+template <class T, int kRowWarps, bool kWide>
 __global__ void __launch_bounds__(kQuantThreads) k_quant_tokens(const T* __restrict__ x, uint32_t rows, uint32_t k, uint64_t ld_x,
                                                                 int8_t* __restrict__ q, uint64_t ld_q, float* __restrict__ scale) {
     __shared__ float part[kQuantThreads / 32];
     tc::grid_trigger();   // a product launched after this kernel sets itself up meanwhile
-    constexpr int N = Vec<T>::kN;
     constexpr uint32_t kRowThreads = 32 * kRowWarps, kRows = kQuantThreads / kRowThreads;
+    constexpr int N = kWide ? Vec<T>::kN : 1, kKeep = kWide ? kHold : kHoldSingle;
     const uint32_t tid = threadIdx.x % kRowThreads;
     const uint64_t row = (uint64_t)blockIdx.x * kRows + threadIdx.x / kRowThreads;
     const bool live = row < rows;   // no early return: the rows of a block share its barrier
     const T* xr = x + (live ? row : 0) * ld_x;
     int8_t* qr = q + (live ? row : 0) * ld_q;
-    const bool wide = ((reinterpret_cast<uintptr_t>(xr) & 15) | (reinterpret_cast<uintptr_t>(qr) & (N - 1))) == 0;
-    const uint32_t kk = live ? k : 0u, nv = wide ? kk / N : 0u;   // whole vectors; the rest one by one
+    const uint32_t kk = live ? k : 0u, nv = kk / N;   // whole vectors; the rest one by one
     float m = 0.f;
-    Vec<T> v[kHold];
+    Vec<T> v[kWide ? kKeep : 1];
+    T one[kWide ? 1 : kKeep];
+    if constexpr (kWide) {
 #pragma unroll
-    for (int i = 0; i < kHold; i++) {
-        const uint32_t j = tid + i * kRowThreads;
-        if (j < nv) v[i].raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
-        else v[i].raw = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kKeep; i++) {
+            const uint32_t j = tid + i * kRowThreads;
+            if (j < nv) v[i].raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
+            else v[i].raw = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kKeep; i++)
+#pragma unroll
+            for (int c = 0; c < N; c++) m = fmaxf(m, fabsf(v[i].get(c)));
+        for (uint32_t j = tid + kKeep * kRowThreads; j < nv; j += kRowThreads) {
+            Vec<T> u;
+            u.raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
+#pragma unroll
+            for (int c = 0; c < N; c++) m = fmaxf(m, fabsf(u.get(c)));
+        }
+        for (uint32_t c = nv * N + tid; c < kk; c += kRowThreads) m = fmaxf(m, fabsf(to_f32(xr[c])));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kKeep; i++) {
+            const uint32_t c = tid + i * kRowThreads;
+            one[i] = c < kk ? xr[c] : T(0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < kKeep; i++) m = fmaxf(m, fabsf(to_f32(one[i])));
+#pragma unroll 4
+        for (uint32_t c = tid + kKeep * kRowThreads; c < kk; c += kRowThreads) m = fmaxf(m, fabsf(to_f32(xr[c])));
     }
-#pragma unroll
-    for (int i = 0; i < kHold; i++)
-#pragma unroll
-        for (int c = 0; c < N; c++) m = fmaxf(m, fabsf(v[i].get(c)));
-    for (uint32_t j = tid + kHold * kRowThreads; j < nv; j += kRowThreads) {
-        Vec<T> u;
-        u.raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
-#pragma unroll
-        for (int c = 0; c < N; c++) m = fmaxf(m, fabsf(u.get(c)));
-    }
-    for (uint32_t c = nv * N + tid; c < kk; c += kRowThreads) m = fmaxf(m, fabsf(to_f32(xr[c])));
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     if (kRowWarps > 1) {
@@ -116,17 +128,27 @@ __global__ void __launch_bounds__(kQuantThreads) k_quant_tokens(const T* __restr
     }
     const float s = row_scale(m);
     const float inv = __fdiv_rn(1.f, s);
+    if constexpr (kWide) {
 #pragma unroll
-    for (int i = 0; i < kHold; i++) {
-        const uint32_t j = tid + i * kRowThreads;
-        if (j < nv) put_quant(qr + (uint64_t)j * N, v[i], inv);
+        for (int i = 0; i < kKeep; i++) {
+            const uint32_t j = tid + i * kRowThreads;
+            if (j < nv) put_quant(qr + (uint64_t)j * N, v[i], inv);
+        }
+        for (uint32_t j = tid + kKeep * kRowThreads; j < nv; j += kRowThreads) {
+            Vec<T> u;
+            u.raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
+            put_quant(qr + (uint64_t)j * N, u, inv);
+        }
+        for (uint32_t c = nv * N + tid; c < kk; c += kRowThreads) qr[c] = (int8_t)quant_one(to_f32(xr[c]), inv);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kKeep; i++) {
+            const uint32_t c = tid + i * kRowThreads;
+            if (c < kk) qr[c] = (int8_t)quant_any(to_f32(one[i]), inv);
+        }
+#pragma unroll 4
+        for (uint32_t c = tid + kKeep * kRowThreads; c < kk; c += kRowThreads) qr[c] = (int8_t)quant_any(to_f32(xr[c]), inv);
     }
-    for (uint32_t j = tid + kHold * kRowThreads; j < nv; j += kRowThreads) {
-        Vec<T> u;
-        u.raw = *reinterpret_cast<const uint4*>(xr + (uint64_t)j * N);
-        put_quant(qr + (uint64_t)j * N, u, inv);
-    }
-    for (uint32_t c = nv * N + tid; c < kk; c += kRowThreads) qr[c] = (int8_t)quant_one(to_f32(xr[c]), inv);
     if (live && tid == 0) scale[row] = s;
 }
 
@@ -362,6 +384,10 @@ k_w8a8_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
         sm.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    } else if (threadIdx.x == 64) {
+        tc::prefetch_map(&map_a);
+        tc::prefetch_map(&map_w);
+        tc::prefetch_map(&map_o);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&sm.tmem)), "r"(kCols));
@@ -496,14 +522,26 @@ k_w8a8_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         tc::bulk_commit();
                     }
                     ob ^= 1;
-                } else {   // any stride and alignment: a row's columns by consecutive lanes
+                } else {   // any stride and alignment: a row's columns by consecutive lanes, eight rows in flight
                     __syncwarp();
-                    for (int r = 0; r < 32 && row0 + r < g.m; r++)
-                        for (int c = lane; c < kBox && n0 + c0 + c < g.n; c += 32) {
-                            const int chunk = c * (int)sizeof(T) / 16, in = c % (16 / (int)sizeof(T));
-                            ((T*)g.out)[(row0 + r) * g.ld_o + n0 + c0 + c] =
-                                reinterpret_cast<const T*>(box + r * 128 + ((chunk ^ (r & 7)) * 16))[in];
-                        }
+                    constexpr int kPer = kBox / 32;
+                    T* o = (T*)g.out + (uint64_t)row0 * g.ld_o + n0 + c0;
+#pragma unroll
+                    for (int rb = 0; rb < 32; rb += 8) {
+                        T y[8][kPer];
+#pragma unroll
+                        for (int r = 0; r < 8; r++)
+#pragma unroll
+                            for (int h = 0; h < kPer; h++) {
+                                const int c = lane + 32 * h, chunk = c * (int)sizeof(T) / 16, in = c % (16 / (int)sizeof(T));
+                                y[r][h] = reinterpret_cast<const T*>(box + (rb + r) * 128 + ((chunk ^ r) * 16))[in];
+                            }
+#pragma unroll
+                        for (int r = 0; r < 8; r++)
+#pragma unroll
+                            for (int h = 0; h < kPer; h++)
+                                if (row0 + rb + r < g.m && n0 + c0 + lane + 32 * h < g.n) o[(uint64_t)(rb + r) * g.ld_o + lane + 32 * h] = y[r][h];
+                    }
                     __syncwarp();
                 }
             }
