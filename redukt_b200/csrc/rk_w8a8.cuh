@@ -279,12 +279,13 @@ __global__ void __launch_bounds__(kFewThreads) k_w8a8_few(Args a, const X* __res
 //
 // Persistent, one CTA per SM: warp 0 brings stages of 128 bytes of K (TMA, 128-byte swizzle; what lies
 // past a matrix's edge arrives as zeros, which add nothing), warp 1 owns TMEM and issues
-// tcgen05.mma kind::i8 (M = 128 tokens, N = BN channels, int32 sums), warps 2-5 read the sums of the
-// previous tile back (tcgen05.ld, thread = token), scale and store them, so two accumulator sets are
+// tcgen05.mma kind::i8 (M = 128 tokens, N = BN channels, int32 sums), warps 2-9 read the sums of the
+// previous tile back (tcgen05.ld, thread = token, every other box of columns), scale and store them, so two accumulator sets are
 // in flight.  Every wait is bounded; on a timeout the CTA sets bit 1 of the error word, drains its
 // copies and frees its TMEM.
 constexpr int kTileM = 128, kTileK = 128;
-constexpr int kTcThreads = 192;
+constexpr int kEpiWarps = 8;
+constexpr int kTcThreads = 64 + 32 * kEpiWarps;
 constexpr long long kWaitCycles = 4000000000ll;   // about 2 s
 
 // Stages: as many as fit beside the rest.  A batch of fewer than 128 tokens stages only its rows (the product
@@ -294,7 +295,7 @@ constexpr size_t kSmemMax = 232448;
 
 template <int BN>
 struct alignas(1024) TcSmem {
-    uint8_t out[4][2][32 * 128];   // each epilogue warp: two boxes of 32 rows x 128 bytes, swizzled
+    uint8_t out[kEpiWarps][32 * 128];   // each epilogue warp: a box of 32 rows x 128 bytes, swizzled
     float ws[BN];
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t tfull[2], tempty[2];
@@ -380,7 +381,7 @@ k_w8a8_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
         for (int i = 0; i < 2; i++) {
             tc::mbar_init(&sm.tfull[i], 1);
-            tc::mbar_init(&sm.tempty[i], 4);
+            tc::mbar_init(&sm.tempty[i], kEpiWarps);
         }
         sm.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -469,26 +470,25 @@ k_w8a8_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const int e = warp - 2, quad = warp & 3;
         constexpr int kBox = 128 / (int)sizeof(T);   // columns of one 128-byte box row
         uint32_t n = 0;
-        int ob = 0;
         tc::grid_wait();
         for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, n++) {
             uint32_t tm, tn;
             tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
             const uint32_t buf = n & 1, n0 = tn * BN, row0 = tm * kTileM + quad * 32, row = row0 + lane;
-            asm volatile("bar.sync 1, 128;" ::: "memory");   // every epilogue warp is done with ws
-            for (int c = threadIdx.x - 64; c < BN; c += 128) sm.ws[c] = n0 + c < g.n ? g.ws[n0 + c] : 0.f;
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");   // every epilogue warp is done with ws
+            for (int c = threadIdx.x - 64; c < BN; c += 32 * kEpiWarps) sm.ws[c] = n0 + c < g.n ? g.ws[n0 + c] : 0.f;
             const float as = row < g.m ? g.as[row] : 0.f;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
             if (!wait_bar(&sm.tfull[buf], (n >> 1) & 1, abort)) break;
             tc::tc_fence_after();
             const uint32_t src = tmem + buf * BN + ((uint32_t)(quad * 32) << 16);
-            for (int c0 = 0; c0 < BN; c0 += kBox) {
+            for (int c0 = (e >> 2) * kBox; c0 < BN; c0 += kEpiWarps / 4 * kBox) {
                 if (n0 + c0 >= g.n || row0 >= g.m) break;
-                uint8_t* box = sm.out[e][ob];
+                uint8_t* box = sm.out[e];
                 // TMA clips a store to 16 bytes: a box that the row's end cuts elsewhere is stored by lanes
                 const bool by_tma = g.tma_out && (n0 + c0 + kBox <= g.n || g.n % (16 / sizeof(T)) == 0);
                 if (g.tma_out) {   // the box's previous store has been read
-                    if (lane == 0) tc::bulk_wait_read<1>();
+                    if (lane == 0) tc::bulk_wait_read<0>();
                     __syncwarp();
                 }
 #pragma unroll
@@ -521,7 +521,6 @@ k_w8a8_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         tc::tma_store_2d(&map_o, (int)(n0 + c0), (int)row0, box);
                         tc::bulk_commit();
                     }
-                    ob ^= 1;
                 } else {   // any stride and alignment: a row's columns by consecutive lanes, eight rows in flight
                     __syncwarp();
                     constexpr int kPer = kBox / 32;
