@@ -84,6 +84,8 @@ int32_t device(Device** out) {
         OP_CK(cudaFuncSetAttribute(rk::plan::k_plan<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::plan::Smem<1024>)));
         OP_CK(cudaFuncSetAttribute(rk::delta::k_delta_scan<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::delta::ScanSmem<64>)));
         OP_CK(cudaFuncSetAttribute(rk::delta::k_delta_scan<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(rk::delta::ScanSmem<128>)));
+        OP_CK((set_chunk_smem<64, float, true>()));
+        OP_CK((set_chunk_smem<64, __nv_bfloat16, true>()));
         OP_CK((set_chunk_smem<64, float, false>()));
         OP_CK((set_chunk_smem<64, __nv_bfloat16, false>()));
         OP_CK((set_chunk_smem<128, float, false>()));
@@ -147,36 +149,45 @@ int32_t delta_args(const char* what, rk::delta::Args& a, const void* d_q, const 
 
 uint64_t seg_floats(uint64_t hv, uint64_t dk, uint64_t dv) { return hv * dk * (2 * dv + dk); }   // b, s_in, M of a segment
 
+// With a block for each SM at most, only a chain's own latency counts: the wide block's steps overlap with the
+// preparation of the next chunk and take about 0.7 of the narrow block's (14 requests of about 106 tokens, 10
+// heads of 128 x 64, bf16: 65 -> 43 us).
+constexpr double kAloneStep = 0.7;
+bool few_blocks(const Device& d, double chains, uint32_t rows) { return chains * (double)ceil_div(rows, 64) <= d.sms; }
+
 // Table blocks per segment, 0 = the requests are not cut.  Estimated time in chunk steps of one block alone
 // on its SM: co-resident blocks slow one another by about 0.4 of a step each, blocks past the
 // resident ones wait for a wave.  The transition pass has the key's rows beside the value's and, with
-// no outputs, steps of about 0.7; a scan step is about 0.5.  Only the requests' mean length is
+// no outputs, steps of about 0.7; a scan step is about 0.4.  Only the requests' mean length is
 // known here.  16,384 tokens of one request, 8 heads of 128: 2.71 ms uncut.
 uint32_t segment_merge(const Device& d, const rk::delta::Args& a, uint32_t dk, uint32_t block, int rows, int resident, uint64_t work_bytes) {
     const auto steps = [&](double blocks) {
         const double k = blocks / d.sms, waves = std::ceil(blocks / (double)(d.sms * resident));
         return waves * (1.0 + 0.4 * (std::max(1.0, std::min(k, (double)resident)) - 1.0));
     };
-    const double slices = (double)ceil_div(a.dv, rows), both = (double)ceil_div(a.dv + dk, rows);
-    double best = 0.8 * (double)a.n_rows / rk::delta::kC / a.n * steps(a.n * (double)a.hv * slices);
+    const double slices = (double)ceil_div(a.dv, rows), both = (double)ceil_div(a.dv + dk, rows), mean = (double)a.n_rows / a.n;
+    const auto alone = [&](double chains, uint32_t state_rows) { return few_blocks(d, chains, state_rows) ? kAloneStep : 1.0; };
+    // where every chain has an SM, the longest decides: several requests' is taken for 1.4 times their mean
+    const double longest = mean * (a.n > 1 && few_blocks(d, (double)a.n * a.hv, a.dv) ? 1.4 : 1.0);
+    double best = 0.8 * alone((double)a.n * a.hv, a.dv) * longest / rk::delta::kC * steps(a.n * (double)a.hv * slices);
     uint32_t merge = 0;
     for (uint32_t m = 1; (uint64_t)m * block * a.n <= a.n_rows; m *= 2) {
-        const uint64_t segs = a.n_rows / ((uint64_t)m * block) + a.n;
-        if (segs * seg_floats(a.hv, dk, a.dv) * 4 > work_bytes) continue;
-        const double chunks = (double)m * block / rk::delta::kC;
-        const double t = chunks * (0.7 * steps(segs * (double)a.hv * both) + steps(segs * (double)a.hv * slices)) + 0.5 * segs / a.n + 1.0;
+        const uint64_t most = a.n_rows / ((uint64_t)m * block) + a.n;
+        if (most * seg_floats(a.hv, dk, a.dv) * 4 > work_bytes) continue;
+        const double chunks = (double)m * block / rk::delta::kC, segs = std::ceil(mean / ((double)m * block));
+        const double t = alone(a.n * segs * a.hv, a.dv + dk) * chunks *
+                             (0.7 * steps(a.n * (segs - 1.0) * a.hv * both) + steps(a.n * segs * a.hv * slices)) + 0.4 * segs + 1.0;
         if (t < best) best = t, merge = m;
     }
     return merge;
 }
 
+// The launches of one shape of block: whole requests (merge 0), or segments of `merge` table blocks.
 template <int DK, class T, bool kWide>
-int32_t launch_chunk(const Device& d, rk::delta::ChunkArgs ca, uint32_t max_blocks, void* d_work, uint64_t work_bytes, cudaStream_t st) {
+int32_t launch_chunk(rk::delta::ChunkArgs ca, uint32_t max_blocks, void* d_work, cudaStream_t st) {
     using namespace rk::delta;
     using Cfg = ChunkCfg<DK, T, kWide>;
     const unsigned slices = (unsigned)ceil_div(ca.a.dv, Cfg::kRows), smem = (unsigned)sizeof(ChunkSmem<DK, T, kWide>);
-    if (ca.blocks && d_work) ca.merge = segment_merge(d, ca.a, DK, ca.block, Cfg::kRows, Cfg::kMinBlocks, work_bytes);
-    else ca.merge = 0;
     if (!ca.merge) {
         k_delta_chunk<DK, T, kWide, 0><<<dim3(slices, ca.a.hv, ca.a.n), Cfg::kThreads, smem, st>>>(ca);
     } else {
@@ -192,13 +203,18 @@ int32_t launch_chunk(const Device& d, rk::delta::ChunkArgs ca, uint32_t max_bloc
     return BACKEND_OK;
 }
 
-// 128 value rows per block where there are that many to fill it, 64 otherwise.
-template <class T>
-int32_t launch_chunk_t(const Device& d, const rk::delta::ChunkArgs& ca, uint32_t dk, uint32_t max_blocks, void* d_work, uint64_t work_bytes,
-                       cudaStream_t st) {
-    if (dk == 64) return launch_chunk<64, T, false>(d, ca, max_blocks, d_work, work_bytes, st);
-    if (ca.a.dv <= 64) return launch_chunk<128, T, false>(d, ca, max_blocks, d_work, work_bytes, st);
-    return launch_chunk<128, T, true>(d, ca, max_blocks, d_work, work_bytes, st);
+// Wide blocks for keys of 128 with more than 64 value rows, and wherever there is a block for each SM at most;
+// narrow ones otherwise.
+template <int DK, class T>
+int32_t launch_chunk_t(const Device& d, rk::delta::ChunkArgs ca, uint32_t max_blocks, void* d_work, uint64_t work_bytes, cudaStream_t st) {
+    using namespace rk::delta;
+    const bool wide = DK == 128 && ca.a.dv > 64;
+    const int rows = wide ? ChunkCfg<DK, T, true>::kRows : ChunkCfg<DK, T, false>::kRows;
+    const int resident = wide ? ChunkCfg<DK, T, true>::kMinBlocks : ChunkCfg<DK, T, false>::kMinBlocks;
+    ca.merge = ca.blocks && d_work ? segment_merge(d, ca.a, DK, ca.block, rows, resident, work_bytes) : 0;
+    const double segs = ca.merge ? std::ceil((double)ca.a.n_rows / ca.a.n / ((double)ca.merge * ca.block)) : 1.0;
+    if (wide || few_blocks(d, ca.a.n * segs * ca.a.hv, ca.a.dv + (ca.merge ? DK : 0))) return launch_chunk<DK, T, true>(ca, max_blocks, d_work, st);
+    return launch_chunk<DK, T, false>(ca, max_blocks, d_work, st);
 }
 
 // ---- 8-bit product ----
@@ -477,8 +493,11 @@ int32_t redukt_b200_delta_chunk(const void* d_q, const void* d_k, const void* d_
     a.cu = d_cu;
     const cudaStream_t st = stream_of(cuda_stream);
     rk::delta::ChunkArgs ca = {a, d_blocks, block, 0, nullptr, nullptr, nullptr};
-    return dtype == REDUKT_DTYPE_F32 ? launch_chunk_t<float>(*d, ca, d_key, max_blocks, d_work, work_bytes, st)
-                                     : launch_chunk_t<__nv_bfloat16>(*d, ca, d_key, max_blocks, d_work, work_bytes, st);
+    if (dtype == REDUKT_DTYPE_F32)
+        return d_key == 64 ? launch_chunk_t<64, float>(*d, ca, max_blocks, d_work, work_bytes, st)
+                           : launch_chunk_t<128, float>(*d, ca, max_blocks, d_work, work_bytes, st);
+    return d_key == 64 ? launch_chunk_t<64, __nv_bfloat16>(*d, ca, max_blocks, d_work, work_bytes, st)
+                       : launch_chunk_t<128, __nv_bfloat16>(*d, ca, max_blocks, d_work, work_bytes, st);
 }
 
 int32_t redukt_b200_quantize_tokens(const void* d_x, int32_t dtype, uint32_t n_tokens, uint32_t k, uint64_t ld_x, int8_t* d_q,
