@@ -303,7 +303,8 @@ int32_t redukt_b200_delta_step(const void* d_q, const void* d_k, const void* d_v
  * log_decay, beta and out belong to request i, whose state is in slot d_slots[i] (arguments
  * otherwise as redukt_b200_delta_step).  n_tokens is the number of rows of the arrays; no row at or
  * above it is touched.  A request without tokens keeps its state (fresh: zero state).  The same
- * call gives the same bits every time; they are near, not equal to, n calls of delta_step.
+ * call gives the same bits every time; they are near, not equal to, n calls of delta_step.  A NaN or
+ * infinity among a request's inputs makes its outputs invalid from the 32 tokens around it on.
  * d_blocks (block, max_blocks) is the plan's block table, used to cut long requests where there are
  * few of them; NULL = never cut (block a multiple of 64, max_blocks at most 65,535 and at least
  * n_tokens / block + n_requests).  d_work on 256 bytes: redukt_b200_delta_work_bytes() let requests be
