@@ -17,9 +17,15 @@
 // chain from U_0 to U_1.
 //
 // Precision: an f32 operand is split into two f16 planes hi + lo after scaling its row by a power of
-// two that puts the row's largest value in [2^14, 2^15): 22 bits of every value down to 2^-28 of that
+// two that puts the row's largest value in [2^14, 2^15): every value to 2^-23 of itself or 2^-39 of that
 // largest, and no overflow.  f32 x f32 is hi hi + hi lo + lo hi; a bf16 k or q is one f16 plane
-// exactly, down to 2^-28 of its row's largest.  Sums are f32.
+// exactly, down to 2^-28 of its row's largest.  Sums are f32.  Against 64 bits the outputs and states of
+// 2,700-token windows are off by 3.7e-7.
+//
+// What bounds it: latency.  A warp's state rows take 64 of its registers (key size 128), so an SM holds 10 to 12
+// warps, each a long chain of short dependent steps; issue slots are 40 % used, the tensor pipe 33-39 %,
+// the shared-memory pipe 53-60 %.  32 windows of 2,700 tokens, 12 heads of 64, f32: 0.66 ms (1.6 TB/s of
+// the bytes it cannot do without); 20,648 ragged tokens, 16 heads of 128, bf16: 0.40 ms (1.0 TB/s).
 #pragma once
 #include <cuda_fp16.h>
 

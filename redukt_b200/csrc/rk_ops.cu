@@ -296,7 +296,8 @@ int32_t launch_tc(const Device& d, const rk::w8::Args& a, cudaStream_t st, bool 
     } else {
         mo = ma;   // never used
     }
-    TcArgs g = {a.as, a.ws, a.out, a.ld_o, a.m, a.n, a.k, (uint32_t)ceil_div(a.m, kTileM), (uint32_t)ceil_div(a.n, BN), rows_a, stages<BN>(rows_a), tma_out, d.err};
+    TcArgs g = {a.as, a.ws, a.out, a.ld_o, a.m, a.n, a.k, (uint32_t)ceil_div(a.m, kTileM), (uint32_t)ceil_div(a.n, BN),
+                rows_a, stages<BN>(rows_a), tma_out, d.err};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)std::min<uint64_t>((uint64_t)g.tiles_m * g.tiles_n, d.sms));
     cfg.blockDim = dim3(kTcThreads);
@@ -369,7 +370,9 @@ int32_t matmul(const Device& d, const rk::w8::Args& a, int32_t out_dtype, cudaSt
 }
 
 uint64_t quant_ld(uint32_t k) { return ceil_div(k, 16) * 16; }
-uint64_t quant_bytes(uint32_t n_tokens, uint32_t k) { return ceil_div((uint64_t)n_tokens * quant_ld(k), 256) * 256 + ceil_div(4ull * n_tokens, 256) * 256; }
+uint64_t quant_bytes(uint32_t n_tokens, uint32_t k) {
+    return ceil_div((uint64_t)n_tokens * quant_ld(k), 256) * 256 + ceil_div(4ull * n_tokens, 256) * 256;
+}
 
 // Arguments of a call packed as 64-bit words, converted to an entry point's parameter types in order.
 template <class P>
@@ -528,7 +531,8 @@ int32_t redukt_b200_w8a8_matmul(const int8_t* d_a, uint64_t ld_a, const float* d
     if (int32_t rc = w8_check("w8a8_matmul", n_tokens, n_out, k, ld_w, d_w, d_w_scale, d_out, out_dtype, ld_out)) return rc;
     if (n_tokens == 0 || n_out == 0) return BACKEND_OK;
     OP_REQUIRE(d_a && d_a_scale, "w8a8_matmul: NULL argument");
-    OP_REQUIRE(ld_a >= k && ld_a % 16 == 0 && aligned(d_a, 16) && aligned(d_a_scale, 4), "w8a8_matmul: int8 rows must start on 16 bytes and hold k values");
+    OP_REQUIRE(ld_a >= k && ld_a % 16 == 0 && aligned(d_a, 16) && aligned(d_a_scale, 4),
+               "w8a8_matmul: int8 rows must start on 16 bytes and hold k values");
     rk::w8::Args a = {d_a, d_a_scale, d_w, d_w_scale, ld_a, ld_w, ld_out, n_tokens, n_out, k, d_out};
     Device* d = nullptr;
     if (int32_t rc = device(&d)) return rc;
