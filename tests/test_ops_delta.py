@@ -228,6 +228,15 @@ def test_chunk_gates(lib, gate, dtype, cut):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gate", list(GATES))
+@pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128)])
+def test_chunk_cut_ragged_requests_and_gates(lib, gate, dtype, dk, dv):
+    """Lengths whose mean is long enough to be cut, with an empty request, one token and a part of a segment among them."""
+    Batch([1300, 0, 1, 700, 70], hk=1, hv=2, dk=dk, dv=dv, dtype=dtype, gate=GATES[gate], seed=dk).check(lib, cut=64)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("beta", list(BETAS))
 @pytest.mark.parametrize("dtype", [DTYPE_F32, DTYPE_BF16])
 def test_chunk_betas(lib, beta, dtype):
