@@ -316,13 +316,14 @@ int32_t launch_tc(const Device& d, const rk::w8::Args& a, cudaStream_t st, bool 
 }
 
 // Width of the tensor-core tile: the one whose waves over the SMs cost least, a tile of BN channels taking as
-// long as BN + 32 (its fill and drain do not shrink with it, and a narrow tile reads more shared memory per
-// product).
+// long as BN + 64 (its fill and drain do not shrink with it, and a narrow tile reads more shared memory per
+// product).  Over 393 random shapes timed at every width, 3 to 15,800 tokens, this is 0.06 % above the best width on
+// the average and 7 % at worst (BN + 32: 0.2 %, 14 %; BN alone: 5.6 %, 90 %).
 int tile_width(uint64_t m, uint64_t n, int sms) {
     int best = 256;
     uint64_t least = ~0ull;
     for (int bn : {256, 128, 64}) {
-        const uint64_t waves = ceil_div(ceil_div(m, rk::w8::kTileM) * ceil_div(n, bn), sms), cost = waves * (bn + 32);
+        const uint64_t waves = ceil_div(ceil_div(m, rk::w8::kTileM) * ceil_div(n, bn), sms), cost = waves * (bn + 64);
         if (cost < least) {
             least = cost;
             best = bn;
